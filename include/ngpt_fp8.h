@@ -39,6 +39,15 @@ extern "C" {
 #define NGPT_W_OUT_IN      0
 #define NGPT_W_IN_OUT      1
 
+#define NGPT_DT_BF16       0     /* element types of the operators that take more than one */
+#define NGPT_DT_F32        1
+
+#define NGPT_ACT_NONE      0     /* activations of ngpt_linear_act: z */
+#define NGPT_ACT_RELU2     1     /* max(z, 0)^2 */
+#define NGPT_ACT_GELU      2     /* z Phi(z), Phi the normal distribution function */
+#define NGPT_ACT_GELU_TANH 3     /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+#define NGPT_ACT_SILU      4     /* z / (1 + exp(-z)) */
+
 #define NGPT_MAX_PREDICT   4   /* n_predict (multi-token prediction depth) supported by the CE kernels */
 
 int ngpt_abi_version(void);
@@ -328,6 +337,71 @@ int ngpt_lmhead_ce_bwd_codes(const void* x_f8, const void* w_f8_vk, const int64_
                              float x_s, float w_s, float grad_s, float grad_scale,
                              float A, float B, float C, void* dx_bf16, void* dw_f32, int w_layout,
                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- matrix product with bias, activation and residual in its epilogue ---------------------------
+ * out [M, N] = residual + act(x [M, K] . w [N, K]^T + bias [N]), bf16 in and out, fp32 in between, rounded once.  bias and residual are nullable.
+ * Row strides in elements; where K % 64 == 0 rows of x and w must start on 16 bytes (otherwise both are copied into the workspace).
+ * Any M, N, K.  pre [M, N] (nullable) receives bf16(x w^T + bias), what the backward of an activation needs. */
+int64_t ngpt_linear_act_fwd_workspace_bytes(int M, int N, int K);
+int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw, const void* bias_bf16,
+                        const void* residual_bf16, int64_t ld_residual, int M, int N, int K, int activation,
+                        void* out_bf16, void* pre_bf16, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Its gradients from dout [M, N] (contiguous; it is the residual's gradient itself): dz = bf16(dout act'(pre)), dx [M, K] = dz w,
+ * dw [N, K] = dz^T x, dbias [N] = sum of dout act'(pre) over the rows.  Each of the three outputs is nullable; pre may be null for
+ * NGPT_ACT_NONE, w without dx, x without dw. */
+int64_t ngpt_linear_act_bwd_workspace_bytes(int M, int N, int K);
+int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw,
+                        int M, int N, int K, int activation, void* dx_bf16, void* dw_bf16, void* dbias_bf16,
+                        void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- per-head norm of queries and keys with the position rotation ---------------------------
+ * y = rot(x * rsqrt(mean(x^2) + eps) * weight) for every head of q [B, T, Hq, D] and k [B, T, Hk, D] (`dtype`), one pass over both.
+ * The first R of a head's D values are rotated as R / 2 pairs (a, b) -> (a cos - b sin, b cos + a sin): pairs (i, i + R / 2), or
+ * (2 i, 2 i + 1) with `interleaved`.  cos_tab / sin_tab [P, R / 2] (`tab_dtype`), a row per position; `positions` [B, T] int32 or
+ * int64 (nullable: the token's index in its sequence, T <= P).  A position outside 0 .. P - 1 makes the token's heads NaN and reads
+ * nothing.  Strides are host arrays in elements: {batch, token, head} for q and k, {batch, token} for positions; the D values of a head are
+ * contiguous.  Weights [D] in `dtype`, nullable.  Outputs are contiguous [B, T, H, D].  2 <= D <= 512, R even, 2 <= R <= D. */
+int ngpt_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                      int B, int T, int Hq, int Hk, int D, int R, const void* cos_tab, const void* sin_tab, int tab_dtype, int P,
+                      const void* positions, int positions_64, const int64_t* pos_strides,
+                      const void* q_weight, const void* k_weight, float eps, int interleaved,
+                      void* q_out, void* k_out, void* stream);
+
+/* Its backward from the incoming gradients (strided like q, k) and the forward's inputs: dq, dk contiguous, and, where given, the weights'
+ * gradients [D] in `dtype` (these need the workspace; per-workgroup sums are added up in a fixed order). */
+int64_t ngpt_qk_norm_rope_bwd_workspace_bytes(int D);
+int ngpt_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_strides, const void* dk_out, const int64_t* dk_strides,
+                          const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
+                          int B, int T, int Hq, int Hk, int D, int R, const void* cos_tab, const void* sin_tab, int tab_dtype, int P,
+                          const void* positions, int positions_64, const int64_t* pos_strides,
+                          const void* q_weight, const void* k_weight, float eps, int interleaved,
+                          void* dq, void* dk, void* dq_weight, void* dk_weight,
+                          void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- distillation from a teacher's top logits --------------------------------------------------
+ * Row by row, z = softcap(logits) / temperature, softcap(l) = A sigmoid((l + B) / C) (C == 0: no softcap), q = softmax(z) over V columns.
+ * ids [T, K] (int32 or int64) and teacher [T, K] fp32 list a teacher's logits of K columns.  p = softmax of the listed teacher / temperature;
+ * or, with teacher_lse [T] (the teacher's log-sum-exp over all of ITS columns at this temperature), p = exp(teacher / temperature - lse),
+ * and the rest of the teacher's mass stands against the rest of the student's:
+ *     losses[t] = row_weight[t] * temperature^2 * ( sum_j p_j (log p_j - log q_idj)  [ + P (log P - log Q) ] ),
+ *     P = max(0, 1 - sum_j p_j) (0 if every column is listed), Q = 1 - sum_j q_idj
+ * Entries whose id is not in 0 .. V - 1 count for nothing; a column listed twice counts as two entries of p and as one column of Q.  A row with no
+ * entry, or of weight 0 (row_weight is nullable), has loss 0 and gradient 0.  K <= 512.
+ * fwd: losses and, if `stats` (ngpt_distill_stats_bytes(T) bytes) is given, what bwd needs.  bwd: grad = d(sum dlosses * losses) / d logits.
+ * fwd_bwd: both at once for dlosses = grad_scale, reading the logits once; V <= ngpt_distill_fused_max_cols(dtype).
+ * logits and grad are `dtype` with row strides ld, ld_grad (elements). */
+int64_t ngpt_distill_stats_bytes(int T);
+int ngpt_distill_fused_max_cols(int dtype);
+int ngpt_distill_fwd(const void* logits, int dtype, int64_t ld, const void* ids, int ids_64, const float* teacher, const float* teacher_lse,
+                     const float* row_weight, int T, int V, int K, float temperature, float A, float B, float C,
+                     float* losses, float* stats, void* stream);
+int ngpt_distill_bwd(const void* logits, int dtype, int64_t ld, const void* ids, int ids_64, const float* teacher, const float* teacher_lse,
+                     const float* row_weight, int T, int V, int K, float temperature, float A, float B, float C,
+                     const float* stats, const float* dlosses, int64_t dlosses_stride, void* grad, int64_t ld_grad, void* stream);
+int ngpt_distill_fwd_bwd(const void* logits, int dtype, int64_t ld, const void* ids, int ids_64, const float* teacher, const float* teacher_lse,
+                         const float* row_weight, int T, int V, int K, float temperature, float A, float B, float C,
+                         float grad_scale, float* losses, void* grad, int64_t ld_grad, void* stream);
 
 #ifdef __cplusplus
 }

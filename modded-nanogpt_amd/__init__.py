@@ -7,6 +7,7 @@ Importing this package registers the operators (torch.ops.nanogpt.*).  The compu
 its absence is an error: there is no fallback implementation.
 """
 from . import _lib, ops                                   # noqa: F401  (registers torch.ops.nanogpt.*)
+from .block import distill_topk, distill_topk_fwd_bwd, linear_act, qk_norm_rope              # noqa: F401
 from .fused import (FusedLinearReLUSquareFunction, FusedSoftcappedCrossEntropy, ReLUSqrdMLP,  # noqa: F401
                     linear_relu_square, quantize_transpose_mlp_down_weights, reduce_mlp_activation_scales,
                     transpose_add, transpose_copy)
@@ -16,4 +17,5 @@ __all__ = [
     "FusedLinearReLUSquareFunction", "FusedSoftcappedCrossEntropy", "ReLUSqrdMLP",
     "linear_relu_square", "transpose_copy", "transpose_add", "quantize_transpose_mlp_down_weights",
     "reduce_mlp_activation_scales", "gemm_fp8_tn", "quant_fp8", "quant_fp8_2d", "mlp_input_quant", "quant_up_weights",
+    "linear_act", "qk_norm_rope", "distill_topk", "distill_topk_fwd_bwd",
 ]

@@ -16,6 +16,7 @@ BENCH_SIGNATURES = {
 E4M3, E5M2 = 0, 1
 W_OUT_IN, W_IN_OUT = 0, 1
 K_CONTIGUOUS, K_ROWS = 0, 1
+DT_BF16, DT_F32 = 0, 1
 MAX_PREDICT = 4
 
 _P, _I, _L, _F = c_void_p, c_int, c_int64, c_float
@@ -71,6 +72,19 @@ SIGNATURES = {
                                       _P, _P, _P, _P, _P, _P, _I, _P, _L, _P]),
     "ngpt_lmhead_ce_bwd_codes": (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _P, _P, _I, _I, _I, _F, _F, _F, _F,
                                       _F, _F, _F, _P, _P, _I, _P, _L, _P]),
+    "ngpt_linear_act_fwd_workspace_bytes": (_L, [_I, _I, _I]),
+    "ngpt_linear_act_fwd": (_I, [_P, _L, _P, _L, _P, _P, _L, _I, _I, _I, _I, _P, _P, _P, _L, _P]),
+    "ngpt_linear_act_bwd_workspace_bytes": (_L, [_I, _I, _I]),
+    "ngpt_linear_act_bwd": (_I, [_P, _P, _P, _L, _P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P]),
+    "ngpt_qk_norm_rope": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P, _F, _I, _P, _P, _P]),
+    "ngpt_qk_norm_rope_bwd_workspace_bytes": (_L, [_I]),
+    "ngpt_qk_norm_rope_bwd": (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P, _F, _I,
+                                   _P, _P, _P, _P, _P, _L, _P]),
+    "ngpt_distill_stats_bytes": (_L, [_I]),
+    "ngpt_distill_fused_max_cols": (_I, [_I]),
+    "ngpt_distill_fwd": (_I, [_P, _I, _L, _P, _I, _P, _P, _P, _I, _I, _I, _F, _F, _F, _F, _P, _P, _P]),
+    "ngpt_distill_bwd": (_I, [_P, _I, _L, _P, _I, _P, _P, _P, _I, _I, _I, _F, _F, _F, _F, _P, _P, _L, _P, _L, _P]),
+    "ngpt_distill_fwd_bwd": (_I, [_P, _I, _L, _P, _I, _P, _P, _P, _I, _I, _I, _F, _F, _F, _F, _F, _P, _P, _L, _P]),
 }
 
 _lib = None

@@ -12,13 +12,15 @@ import pathlib
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = pathlib.Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libngpt_fp8.so"
 BENCH_LIB_PATH = LIB_DIR / "libngpt_fp8_bench.so"     # + the timing aids behind NGPT_BENCH_BUILD, for measurements only
-SOURCES = ["gemm_api.hip", "quant.hip", "ce.hip", "mlp_aux.hip", "bench_kernels.hip"]   # the last one is empty without NGPT_BENCH_BUILD
+SOURCES = ["gemm_api.hip", "quant.hip", "ce.hip", "mlp_aux.hip", "linear.hip", "qk_rope.hip", "distill.hip", "bench_kernels.hip"]   # the last one is empty without NGPT_BENCH_BUILD
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
@@ -35,14 +37,7 @@ def hipcc_path() -> str:
     raise RuntimeError("hipcc not found (set HIPCC or add /opt/rocm/bin to PATH)")
 
 
-def build(verbose: bool = True, bench: bool = False) -> pathlib.Path:
-    """Compile every HIP source into one shared library; always recompiles.  `bench`: the measurement build."""
-    LIB_DIR.mkdir(exist_ok=True)
-    srcs = [str(CSRC / s) for s in SOURCES if (CSRC / s).exists()]
-    out = BENCH_LIB_PATH if bench else LIB_PATH
-    tmp = out.with_suffix(".so.tmp")
-    cmd = [hipcc_path(), *HIPCC_FLAGS, *(["-DNGPT_BENCH_BUILD"] if bench else []), "-I", str(PKG.parent / "include"),
-           "-o", str(tmp), *srcs]
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print("+", " ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -53,6 +48,21 @@ def build(verbose: bool = True, bench: bool = False) -> pathlib.Path:
         raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{err}")
     if verbose and err.strip():
         print(err, file=sys.stderr)
+
+
+def build(verbose: bool = True, bench: bool = False) -> pathlib.Path:
+    """Compile every HIP source into one shared library; always recompiles.  `bench`: the measurement build."""
+    LIB_DIR.mkdir(exist_ok=True)
+    srcs = [str(CSRC / s) for s in SOURCES if (CSRC / s).exists()]
+    out = BENCH_LIB_PATH if bench else LIB_PATH
+    tmp = out.with_suffix(".so.tmp")
+    flags = [*[f for f in HIPCC_FLAGS if f != "-shared"], *(["-DNGPT_BENCH_BUILD"] if bench else []), "-I", str(PKG.parent / "include")]
+    with tempfile.TemporaryDirectory() as objdir:
+        # one object a source, compiled side by side, then one link
+        objs = [str(pathlib.Path(objdir) / (pathlib.Path(s).stem + ".o")) for s in srcs]
+        with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1, 8)) as pool:
+            list(pool.map(lambda so: _run([hipcc_path(), *flags, "-c", "-o", so[1], so[0]], verbose), zip(srcs, objs)))
+        _run([hipcc_path(), *HIPCC_FLAGS, "-o", str(tmp), *objs], verbose)
     os.replace(tmp, out)
     return out
 

@@ -173,6 +173,23 @@ int gemm_balanced_bf16(const void* A, int fa, int64_t lda, const void* B, int fb
     return check_launch("gemm_balanced_bf16");
 }
 
+// C[R, C] = A . B^T on bf16 operands (K in bytes), of which the first R_out rows and C_out columns are written: operands may be padded
+// beyond the result, by less than a tile.  A result whose rows do not start on 8 bytes is written without split tiles.
+int gemm_bf16_clipped(const void* A, int fa, int64_t lda, const void* B, int fb, int64_t ldb, int R, int C, int K, int R_out, int C_out,
+                      void* out_bf16, int64_t ldc, float* part32, hipStream_t st) {
+    if (R <= 0 || C <= 0 || K <= 0 || K % 128 || R_out > R || C_out > C || R - R_out >= MainCfg::BM || C - C_out >= MainCfg::BN)
+        return fail(NGPT_EALIGN, "gemm_bf16_clipped: R=%d C=%d K=%d of which %d x %d", R, C, K, R_out, C_out);
+    BalancePlan p = plan_balance(R, C, K);
+    if (C_out % 4 || ldc % 4 || ((uintptr_t)out_bf16 & 7)) { p.splits = 1; p.full = p.tiles; p.rem = 0; }
+    if (p.splits > 1 && (!part32 || p.rem * p.splits > kMaxGrid)) return fail(NGPT_EINVAL, "gemm_bf16_clipped: split tiles need the fp32 scratch tiles");
+    ProfileScope prof(g_gemm_slot, st);
+    GemmOperands g{(const uint8_t*)A, (const uint8_t*)B, lda, ldb, R, C, K, p.splits, 0, p.full, 0};
+    EpiStoreBf16 epi{(uint16_t*)out_bf16, ldc, 1.0f, R_out, C_out, part32, false, 0, nullptr, nullptr};
+    if (int e = launch_gemm<MainCfg>(g, fa, fb, epi, st)) return e;
+    if (p.splits > 1) rem_tiles_kernel<uint16_t><<<dim3(p.rem, kRemSlices), 256, 0, st>>>(part32, p.splits, (uint16_t*)out_bf16, ldc, R_out, C_out, p.full);
+    return check_launch("gemm_bf16_clipped");
+}
+
 // fp32 output.  accumulate: every tile adds into `out` (which the caller initialised) with atomics; otherwise whole
 // tiles are stored and the split tiles are added up from their parts in part32.
 int gemm_balanced_f32(const void* A, int fa, int64_t lda, const void* B, int fb, int64_t ldb, int layout, int R, int C, int K,
