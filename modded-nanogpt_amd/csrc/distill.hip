@@ -8,13 +8,14 @@
 //   (F = 1 without the rest), and the softcap's slope A / C sigma (1 - sigma) on top.
 // Entries whose id is not a column are ignored; a row without entries has loss 0 and gradient 0; a row of weight 0 too.
 //
-// A row is 100 KB (50304 bf16), read once and, with a gradient, written once: the bound is memory.  One workgroup of 1024
-// threads owns a row at a time; every thread keeps its pieces of the row in registers from the load to the store.
+// A row is 100 KB (50304 bf16), read once and, with a gradient, written once: the bound is memory.  One workgroup of 960 + 64
+// threads owns a row at a time; every one of the 960 keeps its pieces of the row in registers from the load to the store.
 //  * the exponentials are taken relative to a reference of the thread's own (its maximum; the cap's upper end with a softcap,
 //    which needs no maximum), so one workgroup reduction of (reference, sum) pairs is all that a row needs;
 //  * what is kept per logit is the gradient up to the row's factor, e or e sigma (1 - sigma), in fp32;
-//  * wave 0 prepares the listed columns of the row meanwhile (normaliser, duplicates, the student's logits there) and hands
-//    every one to the thread that owns the column, by a list in LDS: each byte of the gradient is stored once.
+//  * a sixteenth wave prepares the listed columns (normaliser, repetitions, the student's logits there) of the NEXT row and hands
+//    every one to the thread that owns the column, by a list in LDS; the owner stores it after the piece it lies in;
+//  * the next row's loads are issued before this row is reduced and written: one barrier a row.
 #include "common.h"
 #include "host_util.h"
 #include <cmath>
@@ -22,8 +23,11 @@
 namespace ngpt {
 namespace {
 
-constexpr int kDistThreads = 1024;
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kDistThreads = 960;                         // threads that hold the row
 constexpr int kDistWaves = kDistThreads / 64;
+constexpr int kDistBlock = kDistThreads + 64;             // and one wave for the listed columns
 constexpr int kDistMaxTop = 512;          // listed columns a row may have (each takes 40 bytes of LDS)
 
 enum : int { DIST_LOSS = 0, DIST_FUSED = 1, DIST_BWD = 2 };
@@ -79,36 +83,60 @@ struct RowSpan {
     }
 };
 
+// Value by value only where a piece lies in the row in part (a loop: it is rare, and code size matters more).
 template <class T>
 __device__ __forceinline__ v4i load_piece(const T* row, int V, const RowSpan& sp, int i) {
     // values outside the row read as -inf
     constexpr int PER = Elem<T>::PER;
     constexpr int kNegInf = sizeof(T) == 2 ? (int)0xff80ff80u : (int)0xff800000u;
     const int c0 = i * PER - sp.shift;             // column of the piece's first value
+    if (c0 >= 0 && c0 + PER <= V) return *(const v4i*)(row + c0);
     v4i w = {kNegInf, kNegInf, kNegInf, kNegInf};
     if (i < sp.pieces) {
-        if (c0 >= 0 && c0 + PER <= V) {
-            w = *(const v4i*)(row + c0);
-        } else {
-#pragma unroll
-            for (int e = 0; e < PER; ++e) {
-                const int c = c0 + e;
-                if (c >= 0 && c < V) {
-                    if constexpr (sizeof(T) == 2) w[e >> 1] = (e & 1) ? (int)(((uint32_t)w[e >> 1] & 0xffffu) | ((uint32_t)row[c] << 16))
-                                                                     : (int)(((uint32_t)w[e >> 1] & 0xffff0000u) | (uint32_t)row[c]);
-                    else w[e] = __float_as_int(row[c]);
-                }
+#pragma unroll 1
+        for (int e = PER - 1; e >= 0; --e) {       // the piece as one 128-bit number, shifted up value by value
+            const int c = c0 + e;
+            const bool in = c >= 0 && c < V;
+            if constexpr (sizeof(T) == 2) {
+                w.w = (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16);
+                w.z = (int)__builtin_amdgcn_alignbit((uint32_t)w.z, (uint32_t)w.y, 16);
+                w.y = (int)__builtin_amdgcn_alignbit((uint32_t)w.y, (uint32_t)w.x, 16);
+                w.x = (int)(((uint32_t)w.x << 16) | (in ? (uint32_t)row[c] : 0xff80u));
+            } else {
+                w.w = w.z;
+                w.z = w.y;
+                w.y = w.x;
+                w.x = in ? __float_as_int(row[c]) : kNegInf;
             }
         }
     }
     return w;
 }
 
+// Where the matrix starts on 16 bytes (AL), rows are accessed through a descriptor of the row's blocks.  Its bounds check replaces the
+// branches (reads past the row's last 4 bytes give 0, writes there are dropped), and a piece's address is one 32-bit offset.  What a row's
+// first and last block hold of its neighbours is read (it is part of the matrix, or of the last value's own 4 bytes) and not used.
+template <class T>
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* row, int V, const RowSpan& sp) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(row - sp.shift), 0, (int)(((sp.shift + V) * sizeof(T) + 3) & ~3u), 0x00020000);
+}
+// A word of a piece: values before `lo` and from `hi` on (counted from the word's first) become -inf.
+template <class T>
+__device__ __forceinline__ int keep_values(int w, int lo, int hi) {
+    if constexpr (sizeof(T) == 4) return lo <= 0 && hi > 0 ? w : (int)0xff800000u;
+    const uint32_t a = lo <= 0 && hi > 0 ? (uint32_t)w & 0xffffu : 0xff80u;
+    const uint32_t b = lo <= 1 && hi > 1 ? (uint32_t)w & 0xffff0000u : 0xff800000u;
+    return (int)(a | b);
+}
+
+template <class T> __device__ __forceinline__ void store_one(T* p, float v);
+template <> __device__ __forceinline__ void store_one<uint16_t>(uint16_t* p, float v) { *p = (uint16_t)cvt_pk_bf16(v, v); }
+template <> __device__ __forceinline__ void store_one<float>(float* p, float v) { *p = v; }
+
 template <class T>
 __device__ __forceinline__ void store_piece(T* row, int V, const RowSpan& sp, int i, const float* g, bool vec) {
     constexpr int PER = Elem<T>::PER;
     const int c0 = i * PER - sp.shift;
-    if (i >= sp.pieces) return;
     if (vec && c0 >= 0 && c0 + PER <= V) {
         if constexpr (sizeof(T) == 2)
             *(v4i*)(row + c0) = (v4i){(int)cvt_pk_bf16(g[0], g[1]), (int)cvt_pk_bf16(g[2], g[3]), (int)cvt_pk_bf16(g[4], g[5]), (int)cvt_pk_bf16(g[6], g[7])};
@@ -116,13 +144,11 @@ __device__ __forceinline__ void store_piece(T* row, int V, const RowSpan& sp, in
             *(v4f*)(row + c0) = (v4f){g[0], g[1], g[2], g[3]};
         return;
     }
+    if (i >= sp.pieces) return;
 #pragma unroll
     for (int e = 0; e < PER; ++e) {
         const int c = c0 + e;
-        if (c >= 0 && c < V) {
-            if constexpr (sizeof(T) == 2) row[c] = (uint16_t)cvt_pk_bf16(g[e], g[e]);
-            else row[c] = g[e];
-        }
+        if (c >= 0 && c < V) store_one<T>(row + c, g[e]);
     }
 }
 
@@ -159,7 +185,7 @@ struct TopLds {
     int any;                         // entries that are columns
 };
 
-// Wave 0: everything about the listed columns that does not need the row's sum.
+// One wave: everything about the listed columns that does not need the row's sum.
 template <class T, bool CAP, bool TAIL>
 __device__ __forceinline__ void prepare_top(const DistArgs& a, int row, const T* lrow, int shift, TopLds& tp, double* td, int lane) {
     constexpr int PER = Elem<T>::PER;
@@ -298,39 +324,75 @@ __device__ __forceinline__ void for_listed(const TopLds& tp, int tid, int seg, F
 // A sum relative to m taken relative to M >= m.  One whose reference is -inf is empty (or NaN, which is kept).
 __device__ __forceinline__ float rescale(float s, float m, float M, float k2) { return m == -INFINITY ? s : s * exp2_hw((m - M) * k2); }
 
-template <class T, int NCH, bool CAP, bool TAIL, int MODE>
-__global__ __launch_bounds__(kDistThreads, MODE == DIST_FUSED ? 4 : 8) void distill_kernel(DistArgs a) {
+template <class T, int NCH, bool CAP, bool TAIL, int MODE, bool AL>
+__global__ __launch_bounds__(kDistBlock, NCH * Elem<T>::PER > 16 ? 4 : 8) void distill_kernel(DistArgs a) {
     constexpr int PER = Elem<T>::PER;
     constexpr int N = NCH * PER;                        // values a thread holds
     constexpr int SEG = NCH * kDistThreads;             // pieces that one sweep over the registers covers
     constexpr float kLn2 = 0.6931471805599453f;
-    __shared__ TopLds top[2];
+    // Three buffers: the list wave works a row ahead, and the others may be one barrier behind it.
+    // A first row's lists are waited for only where they are used ahead of the row's own barrier.
+    constexpr bool kListsFirst = TAIL || MODE == DIST_BWD;
+    constexpr bool kAhead = N <= 16;                    // registers for a second sweep's loads
+    __shared__ TopLds top[3];
     __shared__ double td[kDistMaxTop];
-    __shared__ float red_m[2][kDistWaves], red_s[2][kDistWaves];
+    __shared__ __attribute__((aligned(16))) float red_m[2][kDistWaves + 1], red_s[2][kDistWaves + 1];      // (the list wave's entry is an empty sum)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int V = a.V;
+    const int step = gridDim.x;
+
+    if (wave == kDistWaves) {
+        // ---- the wave of the listed columns ----
+        if (lane < 2) {
+            red_m[lane][kDistWaves] = -INFINITY;
+            red_s[lane][kDistWaves] = 0.0f;
+        }
+        for (int i = lane; i < kDistThreads; i += 64) top[0].head[i] = top[1].head[i] = top[2].head[i] = -1;
+        auto prepare = [&](int row, int buf) {
+            if (row >= a.T) return;
+            const T* lrow = (const T*)a.logits + (int64_t)row * a.ld;
+            prepare_top<T, CAP, TAIL>(a, row, lrow, RowSpan(lrow, V).shift, top[buf], td, lane);
+        };
+        prepare(blockIdx.x, 0);
+        if constexpr (kListsFirst) __syncthreads();
+        int buf = 1;
+        for (int row = blockIdx.x; row < a.T; row += step) {
+            prepare(row + step, buf);
+            buf = buf == 2 ? 0 : buf + 1;
+            __syncthreads();
+        }
+        return;
+    }
+
+    // ---- the waves that hold the row ----
     // the cap is the largest z: no maximum is needed.  A value of -inf in place of one that is not summed adds exactly this:
     const float pad = CAP ? exp2_hw(-a.k2) : 0.0f;
-
-    top[0].head[tid] = -1;
-    top[1].head[tid] = -1;
-    __syncthreads();
-
-    int par = 0;
-    for (int row = blockIdx.x; row < a.T; row += gridDim.x, par ^= 1) {
+    v4i raw[NCH];
+    auto load_seg = [&](int row, int seg, v4i (&raw)[NCH]) {
         const T* const lrow = (const T*)a.logits + (int64_t)row * a.ld;
-        const RowSpan sp(lrow, V);
-        TopLds& tp = top[par];
-        const float weight = a.weight ? a.weight[row] : 1.0f;
-        v4i raw[NCH];
-        auto load_seg = [&](int seg) {
+        int t = tid;
+        asm volatile("" : "+v"(t));          // offsets are rebuilt here: kept across the row they would be spilled
+        if constexpr (AL) {
+            const auto buf = row_buffer(lrow, V, RowSpan(lrow, V));
 #pragma unroll
-            for (int s = 0; s < NCH; ++s) raw[s] = load_piece<T>(lrow, V, sp, seg * SEG + s * kDistThreads + tid);
-        };
-        load_seg(0);
-        if (wave == 0) prepare_top<T, CAP, TAIL>(a, row, lrow, sp.shift, tp, td, lane);
-        if (TAIL || MODE == DIST_BWD) __syncthreads();
+            for (int s = 0; s < NCH; ++s) {
+                const int i = seg * SEG + s * kDistThreads + t;
+                raw[s] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(buf, i * 16, 0, 0));
+            }
+        } else {
+            const RowSpan sp(lrow, V);
+#pragma unroll
+            for (int s = 0; s < NCH; ++s) raw[s] = load_piece<T>(lrow, V, sp, seg * SEG + s * kDistThreads + t);
+        }
+    };
+    if ((int)blockIdx.x < a.T) load_seg(blockIdx.x, 0, raw);
+    if constexpr (kListsFirst) __syncthreads();
 
+    int par = 0, buf = 0;
+    for (int row = blockIdx.x; row < a.T; row += step, par ^= 1, buf = buf == 2 ? 0 : buf + 1) {
+        const RowSpan sp((const T*)a.logits + (int64_t)row * a.ld, V);
+        TopLds& tp = top[buf];
+        const float weight = a.weight ? a.weight[row] : 1.0f;
         float d[MODE == DIST_LOSS ? 1 : N];
         float m = CAP ? 1.0f : -INFINITY, S = 0.0f;         // reference, in units of z_arg, and the sum relative to it
         int skipped = 0;                                // values of this thread that are not summed
@@ -338,6 +400,22 @@ __global__ __launch_bounds__(kDistThreads, MODE == DIST_FUSED ? 4 : 8) void dist
         // Exponentials of one sweep, relative to `m`, and (forward) their sum.  With the rest of the teacher's mass in play
         // the sum is over the columns that are not listed: those are set to -inf first.
         auto sweep = [&](int seg) {
+            if constexpr (AL && MODE != DIST_BWD) {      // what was read outside the row
+                constexpr int WORD = 4 / sizeof(T);
+                int t = tid;
+                asm volatile("" : "+v"(t));
+                if (seg == 0 && wave == 0 && sp.shift > 0) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) raw[0][i] = t == 0 ? keep_values<T>(raw[0][i], sp.shift - i * WORD, WORD) : raw[0][i];
+                }
+#pragma unroll
+                for (int s = 0; s < NCH; ++s)
+                    if (seg * SEG + (s + 1) * kDistThreads >= sp.pieces) {       // the row's last piece, and none
+                        const int left = V + sp.shift - (seg * SEG + s * kDistThreads + t) * PER;
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) raw[s][i] = keep_values<T>(raw[s][i], 0, left - i * WORD);
+                    }
+            }
             if constexpr (MODE != DIST_BWD) {
                 if constexpr (TAIL) {
                     for_listed<NCH, PER>(tp, tid, seg, [&](int, int idx) {
@@ -351,7 +429,12 @@ __global__ __launch_bounds__(kDistThreads, MODE == DIST_FUSED ? 4 : 8) void dist
                             }
                     });
                 }
-                if constexpr (CAP) {
+                if constexpr (CAP && AL) {
+                    const int mine = max(0, min((sp.pieces - seg * SEG - tid + kDistThreads - 1) / kDistThreads, NCH));       // pieces that exist
+                    skipped += PER * (NCH - mine);
+                    if (tid == 0 && seg == 0) skipped += sp.shift;
+                    if (mine > 0 && seg * SEG + (mine - 1) * kDistThreads + tid == sp.pieces - 1) skipped += sp.pieces * PER - sp.shift - V;
+                } else if constexpr (CAP) {
 #pragma unroll
                     for (int s = 0; s < NCH; ++s) {
                         const int c0 = (seg * SEG + s * kDistThreads + tid) * PER - sp.shift;
@@ -374,29 +457,78 @@ __global__ __launch_bounds__(kDistThreads, MODE == DIST_FUSED ? 4 : 8) void dist
                 const float arg = z_arg<CAP>(Elem<T>::at(raw[i / PER], i % PER), a);
                 const float ex = rel_exp<CAP>(arg, ref, a.k2);
                 if constexpr (MODE != DIST_BWD) S += ex;
-                if constexpr (MODE != DIST_LOSS) d[i] = CAP ? ex * (arg * (1.0f - arg)) : ex;
+                if constexpr (MODE != DIST_LOSS) {
+                    const float u = ex * arg;
+                    d[i] = CAP ? __builtin_fmaf(-u, arg, u) : ex;
+                    asm volatile("" : "+v"(d[i]));       // here and now: moved behind the barrier (as the sum's additions would be) it keeps two values alive
+                }
+                if (i % 8 == 7) {
+                    asm volatile("" : "+v"(S));
+                    __builtin_amdgcn_sched_barrier(0);      // eight chains at a time: more would not fit the registers
+                }
             }
         };
-        // Gradient of one sweep: f times what the thread holds; listed columns from their own statistics.
+        // Gradient of one sweep: f times what the thread holds; then the listed columns, from their own statistics, by the same
+        // thread (its stores to one address stay in order).
         auto emit = [&](int seg, float f, float base, float ref, float inv_sum, bool none) {
             T* const grow = (T*)a.grad + (int64_t)row * a.ldg;
-            if (none) {
+            int t = tid;
+            asm volatile("" : "+v"(t));
+            if constexpr (AL) {
+                const auto buf = row_buffer(grow, V, sp);
+                const bool ragged = (V + sp.shift) % PER != 0;
 #pragma unroll
-                for (int i = 0; i < N; ++i) d[i] = 0.0f;
+                for (int s = 0; s < NCH; ++s) {
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) d[s * PER + e] = none ? 0.0f : d[s * PER + e] * f;
+                    const float* g = &d[s * PER];
+                    u32x4 w;
+                    if constexpr (sizeof(T) == 2) w = (u32x4){cvt_pk_bf16(g[0], g[1]), cvt_pk_bf16(g[2], g[3]), cvt_pk_bf16(g[4], g[5]), cvt_pk_bf16(g[6], g[7])};
+                    else w = (u32x4){__float_as_uint(g[0]), __float_as_uint(g[1]), __float_as_uint(g[2]), __float_as_uint(g[3])};
+                    const int i = seg * SEG + s * kDistThreads + t;
+                    // pieces that are the row's in part: out of bounds here, value by value below
+                    const bool part = (i == 0 && sp.shift > 0) || (i == sp.pieces - 1 && ragged);
+                    __builtin_amdgcn_raw_buffer_store_b128(w, buf, part ? 0x7ffffff0 : i * 16, 0, 0);
+                }
+#pragma unroll
+                for (int s = 0; s < NCH; ++s) {
+                    const int first = seg * SEG + s * kDistThreads;
+                    if ((first == 0 && sp.shift > 0) || (ragged && first < sp.pieces && first + kDistThreads >= sp.pieces)) {
+                        const int i = first + t;
+                        if ((i == 0 && sp.shift > 0) || (i == sp.pieces - 1 && ragged)) {
+#pragma unroll
+                            for (int e = 0; e < PER; ++e) {
+                                const int c = i * PER + e - sp.shift;
+                                if (c >= 0 && c < V) store_one<T>(grow + c, d[s * PER + e]);
+                            }
+                        }
+                    }
+                }
             } else {
 #pragma unroll
-                for (int i = 0; i < N; ++i) d[i] *= f;
-                for_listed<NCH, PER>(tp, tid, seg, [&](int e, int idx) {
+                for (int s = 0; s < NCH; ++s) {
+                    float g[PER];
+#pragma unroll
+                    for (int e = 0; e < PER; ++e) g[e] = none ? 0.0f : d[s * PER + e] * f;
+                    store_piece<T>(grow, V, sp, seg * SEG + s * kDistThreads + t, g, a.vec_grad != 0);
+                }
+            }
+            if (!none)
+                for_listed<NCH, PER>(tp, tid, seg, [&](int e, int) {
                     const float arg = tp.arg[e];
                     const float q = rel_exp<CAP>(arg, ref, a.k2) * inv_sum;
-                    const float v = base * (q * (tp.sum_p + tp.rest_p) - tp.p[e]) * (CAP ? arg * (1.0f - arg) : 1.0f);
-#pragma unroll
-                    for (int i = 0; i < N; ++i) d[i] = i == idx ? v : d[i];
+                    store_one<T>(grow + (tp.pos[e] - sp.shift), base * (q * (tp.sum_p + tp.rest_p) - tp.p[e]) * (CAP ? arg * (1.0f - arg) : 1.0f));
                 });
-            }
+        };
+
+        // The sweep behind this one, of this row or of the next: requested before this one is worked on.
+        auto load_ahead = [&](int seg, v4i (&next)[NCH]) {
+            if (MODE != DIST_FUSED && seg + 1 < segs) load_seg(row, seg + 1, next);
+            else if (row + step < a.T) load_seg(row + step, 0, next);
+        };
+        auto take = [&](const v4i (&next)[NCH]) {
 #pragma unroll
-            for (int s = 0; s < NCH; ++s)
-                store_piece<T>(grow, V, sp, seg * SEG + s * kDistThreads + tid, &d[s * PER], a.vec_grad != 0);
+            for (int s = 0; s < NCH; ++s) raw[s] = next[s];
         };
 
         if constexpr (MODE == DIST_BWD) {
@@ -405,16 +537,26 @@ __global__ __launch_bounds__(kDistThreads, MODE == DIST_FUSED ? 4 : 8) void dist
             const bool none = tp.any == 0 || weight == 0.0f;
             m = st.ref;
             for (int seg = 0; seg < segs; ++seg) {
-                if (seg) load_seg(seg);
+                v4i next[NCH];
+                load_ahead(seg, next);
                 sweep(seg);
                 emit(seg, base * st.inv_sum * (tp.sum_p + tp.rest_p - st.rest_ratio), base, st.ref, st.inv_sum, none);
+                take(next);
             }
+            tp.head[tid] = -1;
+            __syncthreads();
         } else {
-            sweep(0);
-            if constexpr (MODE == DIST_LOSS) {
-                for (int seg = 1; seg < segs; ++seg) {
-                    load_seg(seg);
+            if constexpr (MODE == DIST_LOSS && kAhead) {
+                for (int seg = 0; seg < segs; ++seg) {
+                    v4i next[NCH];
+                    load_ahead(seg, next);
                     sweep(seg);
+                    take(next);
+                }
+            } else {
+                for (int seg = 0; seg < (MODE == DIST_LOSS ? segs : 1); ++seg) {
+                    sweep(seg);
+                    load_ahead(seg, raw);        // in flight while this row is reduced and written
                 }
             }
             if constexpr (CAP) S = __builtin_fmaf(-(float)skipped, pad, S);
@@ -425,12 +567,24 @@ __global__ __launch_bounds__(kDistThreads, MODE == DIST_FUSED ? 4 : 8) void dist
                 red_s[par][wave] = ws;
             }
             __syncthreads();
-            float M = red_m[par][0];
-#pragma unroll
-            for (int w = 1; w < kDistWaves; ++w) M = fmaxf(M, red_m[par][w]);
+            // four waves at a time: the values of the row fill the registers
+            static_assert((kDistWaves + 1) % 4 == 0, "whole quadruples");
+            float M = m;
+            if constexpr (!CAP) {
+                M = -INFINITY;
+#pragma unroll 1
+                for (int w = 0; w < kDistWaves + 1; w += 4) {
+                    const v4f x = *(const v4f*)&red_m[par][w];
+                    M = fmaxf(M, fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])));
+                }
+            }
             float sum = 0.0f;
+#pragma unroll 1
+            for (int w = 0; w < kDistWaves + 1; w += 4) {
+                const v4f x = *(const v4f*)&red_m[par][w], y = *(const v4f*)&red_s[par][w];
 #pragma unroll
-            for (int w = 0; w < kDistWaves; ++w) sum += rescale(red_s[par][w], red_m[par][w], M, a.k2);
+                for (int q = 0; q < 4; ++q) sum += CAP ? y[q] : rescale(y[q], x[q], M, a.k2);
+            }
             float rest_ratio = 0.0f, p_logq = 0.0f;
             if constexpr (TAIL) {
                 // the sum so far is Q's; with the listed columns it is the row's
@@ -455,8 +609,8 @@ __global__ __launch_bounds__(kDistThreads, MODE == DIST_FUSED ? 4 : 8) void dist
                 const float base = weight * a.tau * a.grad_scale * a.slope;
                 emit(0, base * inv_sum * rescale(1.0f, m, M, a.k2) * (tp.sum_p + tp.rest_p - rest_ratio), base, M, inv_sum, none);
             }
+            tp.head[tid] = -1;      // filled again three rows on, two barriers from here
         }
-        tp.head[tid] = -1;          // wave 0 fills this buffer again two rows on, behind the next row's barrier
     }
 }
 
@@ -464,8 +618,12 @@ template <class T, int NCH, bool CAP, bool TAIL, int MODE>
 int launch_distill(const DistArgs& a, hipStream_t st) {
     const int cus = num_cus();
     if (cus <= 0) return fail(NGPT_EINVAL, "no HIP device");
-    const int resident = cus * (MODE == DIST_FUSED ? 1 : 2);
-    distill_kernel<T, NCH, CAP, TAIL, MODE><<<a.T < resident ? a.T : resident, kDistThreads, 0, st>>>(a);
+    const int resident = cus * (NCH * Elem<T>::PER > 16 ? 1 : 2);
+    const int grid = a.T < resident ? a.T : resident;
+    if (((uintptr_t)a.logits & 15) == 0 && (MODE == DIST_LOSS || a.vec_grad))
+        distill_kernel<T, NCH, CAP, TAIL, MODE, true><<<grid, kDistBlock, 0, st>>>(a);
+    else
+        distill_kernel<T, NCH, CAP, TAIL, MODE, false><<<grid, kDistBlock, 0, st>>>(a);
     return check_launch("distill_kernel");
 }
 
@@ -474,13 +632,16 @@ template <class T> int most_pieces(int V) { return V / Elem<T>::PER + 2; }
 
 template <class T, bool CAP, bool TAIL>
 int run_distill(const DistArgs& a, int mode, hipStream_t st) {
-    if (mode == DIST_LOSS) return launch_distill<T, 2, CAP, TAIL, DIST_LOSS>(a, st);
-    if (mode == DIST_BWD) return launch_distill<T, 2, CAP, TAIL, DIST_BWD>(a, st);
+    constexpr int BIG = sizeof(T) == 2 ? 7 : 14;        // pieces a thread: 56 values
+    // Loss or gradient alone: two workgroups a compute unit in short sweeps; with no more rows than compute units a row's whole
+    // latency counts, and the wide sweep has all of the row in flight at once.
+    const bool few = a.T <= num_cus();
+    if (mode == DIST_LOSS) return few ? launch_distill<T, BIG, CAP, TAIL, DIST_LOSS>(a, st) : launch_distill<T, 16 / Elem<T>::PER, CAP, TAIL, DIST_LOSS>(a, st);
+    if (mode == DIST_BWD) return launch_distill<T, 16 / Elem<T>::PER, CAP, TAIL, DIST_BWD>(a, st);
     // the row in registers: 16, 32 or 56 values a thread
-    constexpr int BIG = sizeof(T) == 2 ? 7 : 14;
     const int pieces = most_pieces<T>(a.V);
-    if (pieces <= 2 * kDistThreads) return launch_distill<T, 2, CAP, TAIL, DIST_FUSED>(a, st);
-    if (pieces <= 4 * kDistThreads) return launch_distill<T, 4, CAP, TAIL, DIST_FUSED>(a, st);
+    if (pieces <= 16 / Elem<T>::PER * kDistThreads) return launch_distill<T, 16 / Elem<T>::PER, CAP, TAIL, DIST_FUSED>(a, st);
+    if (pieces <= 32 / Elem<T>::PER * kDistThreads) return launch_distill<T, 32 / Elem<T>::PER, CAP, TAIL, DIST_FUSED>(a, st);
     return launch_distill<T, BIG, CAP, TAIL, DIST_FUSED>(a, st);
 }
 // Columns of a row that fits the registers wherever it starts
