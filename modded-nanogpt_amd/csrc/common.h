@@ -203,6 +203,28 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
+// Sum over p of part[p * stride + col] for 32 columns by a workgroup of 1024 threads (thread = 32 * group + column), in a fixed order:
+// group g adds p = g, g + 32, ..., then group 0 adds the groups.  The result is thread 0 .. 31's; `red` is 32 x 33 floats of LDS.
+constexpr int kColSumThreads = 1024;
+__device__ __forceinline__ float col_sum32(const float* __restrict__ part, int parts, int64_t stride, int col, bool live, float (*red)[33]) {
+    const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
+    float v = 0.0f;
+    if (live) {
+        int p = g;
+        for (; p + 96 < parts; p += 128) {        // four loads in flight
+            const float a0 = part[p * stride + col], a1 = part[(p + 32) * stride + col];
+            const float a2 = part[(p + 64) * stride + col], a3 = part[(p + 96) * stride + col];
+            v += (a0 + a1) + (a2 + a3);
+        }
+        for (; p < parts; p += 32) v += part[p * stride + col];
+    }
+    red[g][c] = v;
+    __syncthreads();
+    if (g == 0)
+        for (int i = 1; i < 32; ++i) v += red[i][c];
+    return v;
+}
+
 // 16-byte global -> LDS copy that bypasses registers.  `lds_wave_base` must be the same for all
 // lanes of the wave; lane l's 16 bytes land at lds_wave_base + 16*l.
 __device__ __forceinline__ void global_to_lds16(const void* gptr, void* lds_wave_base) {

@@ -301,19 +301,12 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restric
     }
 }
 
-// out[c] = bf16(sum over p of part[p][c]), 32 columns a workgroup, parts in a fixed order
-__global__ __launch_bounds__(256) void col_sum_kernel(const float* __restrict__ part, int parts, int N, uint16_t* __restrict__ out) {
-    __shared__ float red[8][32];
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
-    float v = 0.0f;
-    if (col < N)
-        for (int p = g; p < parts; p += 8) v += part[(int64_t)p * N + col];
-    red[g][c] = v;
-    __syncthreads();
-    if (g == 0 && col < N) {
-        for (int i = 1; i < 8; ++i) v += red[i][c];
-        out[col] = (uint16_t)cvt_pk_bf16(v, v);
-    }
+// out[c] = bf16(sum over p of part[p][c]), 32 columns a workgroup
+__global__ __launch_bounds__(kColSumThreads) void col_sum_kernel(const float* __restrict__ part, int parts, int N, uint16_t* __restrict__ out) {
+    __shared__ float red[32][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+    const float v = col_sum32(part, parts, N, col, col < N, red);
+    if (threadIdx.x < 32 && col < N) out[col] = (uint16_t)cvt_pk_bf16(v, v);
 }
 
 int64_t up64(int64_t n) { return (n + 63) / 64 * 64; }
@@ -463,7 +456,7 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
         }
         if (int e = check_launch("act_grad_kernel")) return e;
         if (dbias_bf16) {
-            col_sum_kernel<<<(N + 31) / 32, 256, 0, st>>>(part, p.sum_rows, N, (uint16_t*)dbias_bf16);
+            col_sum_kernel<<<(N + 31) / 32, kColSumThreads, 0, st>>>(part, p.sum_rows, N, (uint16_t*)dbias_bf16);
             if (int e = check_launch("col_sum_kernel")) return e;
         }
     }

@@ -14,6 +14,7 @@
 // which stay in registers while the wave walks the token's heads.  U steps of loads are issued before the first is used.
 #include "common.h"
 #include "host_util.h"
+#include <algorithm>
 
 namespace ngpt {
 namespace {
@@ -32,8 +33,6 @@ struct RopeArgs {
     int B, T, Hq, Hk, D, R, P;
     int pos64, tab_bf16, interleaved;
     float eps;
-    int chunks;                    // head chunks per token
-    int64_t items;                 // B * T * chunks
 };
 
 constexpr int kRopeThreads = 256;
@@ -100,161 +99,179 @@ __device__ __forceinline__ void store8(T* p, const float (&x)[8], int n) {
     }
 }
 
-// Sum over the LPR lanes of a row; every lane gets it.
+// Sum over the LPR lanes of a row; every lane gets it.  Inside 16 lanes by lane permutations of the vector pipe.
+template <int CTRL>
+__device__ __forceinline__ float permuted(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 template <int LPR>
 __device__ __forceinline__ float group_sum(float v) {
-#pragma unroll
-    for (int o = LPR / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    v += permuted<0xb1>(v);                        // lanes 1 0 3 2
+    v += permuted<0x4e>(v);                        // lanes 2 3 0 1
+    v += permuted<0x141>(v);                       // mirrored inside 8
+    if (LPR >= 16) v += permuted<0x140>(v);        // mirrored inside 16
+    if (LPR >= 32) v += __shfl_xor(v, 16, 64);
+    if (LPR >= 64) v += __shfl_xor(v, 32, 64);
     return v;
 }
 
-// Partner of each of the lane's values in its rotated pair (anything for values that are not rotated).
-// AL: R / 2 (pairs of halves) is a multiple of 8, so the partners are the 8 values of one other lane.  Otherwise the
-// row goes through the wave's own LDS block; LDS operations of one wave execute in order.
-template <int LPR, bool AL>
-__device__ __forceinline__ void partners(const float (&x)[8], float (&y)[8], int sub, int lane, int R, int interleaved, float* lds) {
-    if (AL && interleaved) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i ^ 1];
-        return;
-    }
-    if (AL) {
-        const int half = R >> 4;                      // lanes per half
-        const int src = sub < half ? lane + half : (sub < 2 * half ? lane - half : lane);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = __shfl(x[i], src, 64);
-        return;
-    }
-    float* row = lds + (lane - sub) * 8;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) row[sub * 8 + i] = x[i];
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int e = sub * 8 + i;
-        const int p = e >= R ? e : (interleaved ? (e ^ 1) : (e < R / 2 ? e + R / 2 : e - R / 2));
-        y[i] = row[p];
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-}
-
-template <class T, int LPR, bool AL, bool BWD, int U>
+// REG: the halves of the rotated part are whole pieces of 8 values (or the pairs are neighbours), so that a value's partner lies in the same
+// place of ONE other lane; rows of the tables then start on 16 bytes.  AL: 16-byte accesses to the heads.
+template <class T, int LPR, bool AL, bool REG, bool BWD, bool W, int U>
 __global__ __launch_bounds__(kRopeThreads) void qk_rope_kernel(RopeArgs a) {
     constexpr int ROWS = 64 / LPR;                    // rows (heads) of a wave
     constexpr int WAVES = kRopeThreads / 64;
-    __shared__ float exch[AL && !BWD ? 1 : WAVES * 512];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr bool LDS = !REG || (BWD && W);
+    __shared__ __attribute__((aligned(16))) float exch[LDS ? WAVES * 512 : 1];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int sub = lane & (LPR - 1), row_in_wave = lane / LPR;
     const int e0 = sub * 8;
     const int n = a.D - e0;                           // values of this lane that exist (<= 0: none)
-    const int H = a.Hq + a.Hk;
+    const int H = a.Hq + a.Hk, half = a.R / 2;
     const float inv_d = 1.0f / (float)a.D;
-    float* const lds = exch + (AL && !BWD ? 0 : wave * 512);
+    float* const row_lds = exch + (LDS ? wave * 512 + (lane - sub) * 8 : 0);
+    const float nan = __uint_as_float(0x7fc00000u);
 
-    float wq[8], wk[8], dwq[8], dwk[8];
+    // lane that holds the partners of this lane's values, and the place of the lane's values in a row of the tables
+    const int src = a.interleaved || e0 >= a.R ? lane : (e0 < half ? lane + half / 8 : lane - half / 8);
+    const int tab0 = a.interleaved ? e0 / 2 : (e0 < half ? e0 : e0 - half);
+
+    float wq[W ? 8 : 1], wk[W ? 8 : 1], dwq[W && BWD ? 8 : 1], dwk[W && BWD ? 8 : 1];
+    if constexpr (W) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const bool have = i < n;
-        wq[i] = a.qw && have ? load1<T>((const T*)a.qw + e0 + i) : 1.0f;
-        wk[i] = a.kw && have ? load1<T>((const T*)a.kw + e0 + i) : 1.0f;
-        dwq[i] = dwk[i] = 0.0f;
+        for (int i = 0; i < 8; ++i) {
+            wq[i] = a.qw && i < n ? load1<T>((const T*)a.qw + e0 + i) : 1.0f;
+            wk[i] = a.kw && i < n ? load1<T>((const T*)a.kw + e0 + i) : 1.0f;
+            if constexpr (BWD) dwq[i] = dwk[i] = 0.0f;
+        }
     }
 
-    for (int64_t item = (int64_t)blockIdx.x * WAVES + wave; item < a.items; item += (int64_t)gridDim.x * WAVES) {
-        const int64_t token = item / a.chunks;
-        const int chunk = (int)(item - token * a.chunks);
-        const int b = (int)(token / a.T), t = (int)(token - (int64_t)b * a.T);
-        const int h_end = min(H, (chunk + 1) * ROWS * U);
-
-        // all rows of this chunk are requested first
-        Raw8<T, AL> rx[U], rg[BWD ? U : 1];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = (chunk * U + u) * ROWS + row_in_wave;
-            const bool live = h < h_end;
-            const bool is_q = h < a.Hq;
-            const T* p = is_q ? (const T*)a.q + (b * a.q_sb + t * a.q_st + h * a.q_sh)
-                              : (const T*)a.k + (b * a.k_sb + t * a.k_st + (h - a.Hq) * a.k_sh);
-            rx[u].load(p + e0, live ? n : 0);
-            if constexpr (BWD) {
-                const T* g = is_q ? (const T*)a.dq + (b * a.dq_sb + t * a.dq_st + h * a.dq_sh)
-                                  : (const T*)a.dk + (b * a.dk_sb + t * a.dk_st + (h - a.Hq) * a.dk_sh);
-                rg[u].load(g + e0, live ? n : 0);
-            }
-        }
-        // cos / sin of the lane's values; sn carries the sign of the partner's term.  A position outside the table reads
-        // nothing and makes the token's heads NaN.
+    const int tokens = a.B * a.T;                     // (fits: checked on the host)
+    for (int token = blockIdx.x * WAVES + wave; token < tokens; token += gridDim.x * WAVES) {
+        const int b = token / a.T, t = token - b * a.T;
+        const T* const q0 = (const T*)a.q + (b * a.q_sb + t * a.q_st);
+        const T* const k0 = (const T*)a.k + (b * a.k_sb + t * a.k_st);
+        const T* const dq0 = BWD ? (const T*)a.dq + (b * a.dq_sb + t * a.dq_st) : nullptr;
+        const T* const dk0 = BWD ? (const T*)a.dk + (b * a.dk_sb + t * a.dk_st) : nullptr;
+        T* const qo = (T*)a.q_out + (int64_t)token * a.Hq * a.D;
+        T* const ko = (T*)a.k_out + (int64_t)token * a.Hk * a.D;
+        // cos / sin of the lane's values; sn carries the sign of the partner's term (forward: a cos - b sin).  A position outside the
+        // tables reads row 0 and makes the token's heads NaN.
         float cs[8], sn[8];
         {
             int64_t pos = t;
             if (a.pos) pos = a.pos64 ? ((const int64_t*)a.pos)[b * a.p_sb + t * a.p_st] : (int64_t)((const int32_t*)a.pos)[b * a.p_sb + t * a.p_st];
             const bool ok = pos >= 0 && pos < a.P;
-            const int half = a.R / 2;
             const int64_t base = (ok ? pos : 0) * half;
+            if (REG && !a.tab_bf16) {
+                const float *c = (const float*)a.cos + base + tab0, *s = (const float*)a.sin + base + tab0;
+                if (e0 < a.R) {
+                    const v4f c0 = *(const v4f*)c, s0 = *(const v4f*)s;
+                    if (a.interleaved) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int e = e0 + i;
-                float c = 1.0f, s = 0.0f;
-                if (e < a.R) {
-                    const int idx = a.interleaved ? e >> 1 : (e < half ? e : e - half);
-                    c = a.tab_bf16 ? load1<uint16_t>((const uint16_t*)a.cos + base + idx) : ((const float*)a.cos)[base + idx];
-                    s = a.tab_bf16 ? load1<uint16_t>((const uint16_t*)a.sin + base + idx) : ((const float*)a.sin)[base + idx];
-                    const bool first = a.interleaved ? !(e & 1) : e < half;
-                    if (first != BWD) s = -s;           // forward: a cos - b sin; backward: a cos + b sin
+                        for (int i = 0; i < 8; ++i) { cs[i] = c0[i / 2]; sn[i] = s0[i / 2]; }
+                    } else {
+                        const v4f c1 = *(const v4f*)(c + 4), s1 = *(const v4f*)(s + 4);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) { cs[i] = c0[i]; cs[4 + i] = c1[i]; sn[i] = s0[i]; sn[4 + i] = s1[i]; }
+                    }
                 }
-                cs[i] = ok ? c : __uint_as_float(0x7fc00000u);
-                sn[i] = s;
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int h = (chunk * U + u) * ROWS + row_in_wave;
-            const bool live = h < h_end;
-            const bool is_q = h < a.Hq;
-            float x[8], y[8], part[8];
-            rx[u].get(x);
-            float ss = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
-            if constexpr (!BWD) {
-                const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (is_q ? wq[i] : wk[i]);
-                partners<LPR, AL>(x, part, sub, lane, a.R, a.interleaved, lds);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(x[i], cs[i], part[i] * sn[i]);
             } else {
-                float g[8];
-                rg[u].get(g);
-                partners<LPR, AL>(g, part, sub, lane, a.R, a.interleaved, lds);
-                float gx = 0.0f;
-                float gn[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    gn[i] = __builtin_fmaf(g[i], cs[i], part[i] * sn[i]);          // gradient of the normalised, weighted head
-                    g[i] = gn[i] * (is_q ? wq[i] : wk[i]);
-                    gx = __builtin_fmaf(g[i], x[i], gx);
-                }
-                const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
-                const float m = group_sum<LPR>(gx) * inv_d * r * r;              // mean(g xn) r
-#pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = __builtin_fmaf(g[i], r, -(x[i] * r * m));
-                if (a.dw_part && live) {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const float d = gn[i] * x[i] * r;
-                        if (is_q) dwq[i] += d;
-                        else dwk[i] += d;
+                    const int e = e0 + i;
+                    if (e < a.R) {
+                        const int64_t at = base + (a.interleaved ? e >> 1 : (e < half ? e : e - half));
+                        cs[i] = a.tab_bf16 ? load1<uint16_t>((const uint16_t*)a.cos + at) : ((const float*)a.cos)[at];
+                        sn[i] = a.tab_bf16 ? load1<uint16_t>((const uint16_t*)a.sin + at) : ((const float*)a.sin)[at];
                     }
                 }
             }
-            if (live) {
-                T* o = is_q ? (T*)a.q_out + (token * a.Hq + h) * a.D : (T*)a.k_out + (token * a.Hk + (h - a.Hq)) * a.D;
-                store8<T, AL>(o + e0, y, n);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int e = e0 + i;
+                const bool first = a.interleaved ? !(e & 1) : e < half;
+                cs[i] = !ok ? nan : (e < a.R ? cs[i] : 1.0f);
+                sn[i] = e < a.R ? (first != BWD ? -sn[i] : sn[i]) : 0.0f;
+            }
+        }
+        for (int s0 = blockIdx.y * U; s0 * ROWS < H; s0 += gridDim.y * U) {
+            // the loads of all steps are issued before the first is used
+            Raw8<T, AL> rx[U], rg[BWD ? U : 1];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int h = (s0 + u) * ROWS + row_in_wave;
+                const bool is_q = h < a.Hq;
+                const int m = h < H ? n : 0;
+                rx[u].load((is_q ? q0 + h * a.q_sh : k0 + (h - a.Hq) * a.k_sh) + e0, m);
+                if constexpr (BWD) rg[u].load((is_q ? dq0 + h * a.dq_sh : dk0 + (h - a.Hq) * a.dk_sh) + e0, m);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int h = (s0 + u) * ROWS + row_in_wave;
+                const bool live = h < H, is_q = h < a.Hq;
+                float x[8], y[8], g[BWD ? 8 : 1], gn[BWD && W ? 8 : 1];
+                rx[u].get(x);
+                float ss = 0.0f, gx = 0.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = __builtin_fmaf(x[i], x[i], ss);
+                // what is turned: forward x (times the weight), backward dy
+                float v[8], part[8];
+                if constexpr (BWD) rg[u].get(v);
+                else
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) v[i] = W ? x[i] * (is_q ? wq[i] : wk[i]) : x[i];
+                if constexpr (REG) {
+                    if (a.interleaved) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) part[i] = v[i ^ 1];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) part[i] = __shfl(v[i], src, 64);
+                    }
+                } else {          // through the wave's own LDS block: LDS operations of one wave execute in order
+                    *(v4f*)(row_lds + e0) = (v4f){v[0], v[1], v[2], v[3]};
+                    *(v4f*)(row_lds + e0 + 4) = (v4f){v[4], v[5], v[6], v[7]};
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const int e = e0 + i;
+                        part[i] = row_lds[e >= a.R ? e : (a.interleaved ? (e ^ 1) : (e < half ? e + half : e - half))];
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                }
+                if constexpr (!BWD) {
+                    const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = r * __builtin_fmaf(v[i], cs[i], part[i] * sn[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        const float turned = __builtin_fmaf(v[i], cs[i], part[i] * sn[i]);      // gradient of the normalised, weighted head
+                        if constexpr (W) gn[i] = turned;
+                        g[i] = W ? turned * (is_q ? wq[i] : wk[i]) : turned;
+                        gx = __builtin_fmaf(g[i], x[i], gx);
+                    }
+                    const float r = rsqrtf(group_sum<LPR>(ss) * inv_d + a.eps);
+                    const float m = group_sum<LPR>(gx) * inv_d * r * r;              // mean(g xn) r
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = r * __builtin_fmaf(-x[i], m, g[i]);
+                    if constexpr (W) {
+                        if (a.dw_part && live) {
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const float d = gn[i] * x[i] * r;
+                                if (is_q) dwq[i] += d;
+                                else dwk[i] += d;
+                            }
+                        }
+                    }
+                }
+                if (live) store8<T, AL>((is_q ? qo + h * a.D : ko + (h - a.Hq) * a.D) + e0, y, n);
             }
         }
     }
-    if constexpr (BWD) {
+    if constexpr (BWD && W) {
         if (a.dw_part) {
             // fixed order: lanes of a wave that hold the same values (xor shuffles), then the waves one after the other
             for (int which = 0; which < 2; ++which) {
@@ -270,72 +287,78 @@ __global__ __launch_bounds__(kRopeThreads) void qk_rope_kernel(RopeArgs a) {
                 for (int d = threadIdx.x; d < a.D; d += kRopeThreads) {
                     float v = 0.0f;
                     for (int w = 0; w < WAVES; ++w) v += exch[w * 512 + d];
-                    a.dw_part[((int64_t)blockIdx.x * 2 + which) * a.D + d] = v;
+                    a.dw_part[(((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * 2 + which) * a.D + d] = v;
                 }
             }
         }
     }
 }
 
-// dw[which][d] = sum over blocks of part[block][which][d], 32 columns a workgroup, 8 row groups added in a fixed order.
+// dw[which][d] = sum over blocks of part[block][which][d], 32 columns a workgroup
 template <class T>
-__global__ __launch_bounds__(256) void rope_dw_kernel(const float* __restrict__ part, int blocks, int D, T* dqw, T* dkw) {
-    __shared__ float red[8][32];
-    const int c = threadIdx.x & 31, g = threadIdx.x >> 5;
-    const int col = blockIdx.x * 32 + c;
-    float v = 0.0f;
-    if (col < 2 * D)
-        for (int b = g; b < blocks; b += 8) v += part[(int64_t)b * 2 * D + col];
-    red[g][c] = v;
-    __syncthreads();
-    if (g == 0 && col < 2 * D) {
-        for (int i = 1; i < 8; ++i) v += red[i][c];
-        T* out = col < D ? dqw : dkw;
-        if (out) {
-            const int d = col < D ? col : col - D;
-            if constexpr (sizeof(T) == 2) out[d] = (uint16_t)cvt_pk_bf16(v, v);
-            else out[d] = v;
-        }
-    }
+__global__ __launch_bounds__(kColSumThreads) void rope_dw_kernel(const float* __restrict__ part, int blocks, int D, T* dqw, T* dkw) {
+    __shared__ float red[32][33];
+    const int col = blockIdx.x * 32 + (threadIdx.x & 31);
+    const float v = col_sum32(part, blocks, 2 * (int64_t)D, col, col < 2 * D, red);
+    if (threadIdx.x >= 32 || col >= 2 * D) return;
+    T* out = col < D ? dqw : dkw;
+    if (!out) return;
+    const int d = col < D ? col : col - D;
+    if constexpr (sizeof(T) == 2) out[d] = (uint16_t)cvt_pk_bf16(v, v);
+    else out[d] = v;
 }
 
 constexpr int kRopeMaxBlocks = 2048;
+constexpr int kRopeSumBlocks = 1024;      // with weight gradients: as many as are resident, each leaves its sums
 
 template <class T, bool BWD>
-int launch_rope(RopeArgs a, bool aligned, int* blocks, hipStream_t st) {      // *blocks: workgroups launched
-    int lpr = 2;
+int launch_rope(RopeArgs a, bool aligned, bool regular, int* blocks, hipStream_t st) {      // *blocks: workgroups launched
+    int lpr = 8;
     while (lpr * 8 < a.D) lpr *= 2;
     const int rows = 64 / lpr, H = a.Hq + a.Hk, cus = num_cus();
     if (cus <= 0) return fail(NGPT_EINVAL, "no HIP device");
     const int steps = (H + rows - 1) / rows;
     const int64_t tokens = (int64_t)a.B * a.T;
-    // Several heads' loads in flight per lane once there are waves enough to fill the compute units without that
-    // (a few tokens: every wave takes one step, so that all of them run at once).
-    const int u = tokens * steps >= (int64_t)cus * 16 ? (BWD ? 2 : 4) : 1;
-    a.chunks = (steps + u - 1) / u;
-    a.items = tokens * a.chunks;
-    int64_t grid = (a.items + 3) / 4;
-    if (grid > kRopeMaxBlocks) grid = kRopeMaxBlocks;
-    auto go = [&](auto kernel) { kernel<<<(int)grid, kRopeThreads, 0, st>>>(a); };
+    // A wave walks all heads of its tokens and has several steps' loads in flight, where there are tokens enough to fill the compute
+    // units; with fewer every step is a wave of its own.  The number of steps that leaves the fewest empty ones, the larger first.
+    const bool many = tokens >= (int64_t)cus * 16;
+    int u = 1;
+    if (many && aligned && regular) {
+        int best = 1 << 30;
+        for (int c = BWD ? 3 : 4; c >= 2; --c) {
+            const int waste = (steps + c - 1) / c * c - steps;
+            if (waste < best) { best = waste; u = c; }
+        }
+    }
+    int64_t gx = (tokens + 3) / 4;
+    const int gy = many ? 1 : std::min(steps, kRopeSumBlocks);
+    const int most = a.dw_part ? kRopeSumBlocks : kRopeMaxBlocks;
+    if (gx * gy > most) gx = most / gy;
+    if (gx < 1) gx = 1;
+    const bool weights = a.qw || a.kw || a.dw_part;
+    const dim3 grid((unsigned)gx, (unsigned)gy);
+    auto go = [&](auto kernel) { kernel<<<grid, kRopeThreads, 0, st>>>(a); };
     auto pick = [&](auto lpr_c) {
         constexpr int L = decltype(lpr_c)::value;
-        if (aligned) {
-            if (u == 1) go(qk_rope_kernel<T, L, true, BWD, 1>);
-            else go(qk_rope_kernel<T, L, true, BWD, BWD ? 2 : 4>);
-        } else {
-            if (u == 1) go(qk_rope_kernel<T, L, false, BWD, 1>);
-            else go(qk_rope_kernel<T, L, false, BWD, BWD ? 2 : 4>);
-        }
+        auto steps_of = [&](auto w_c) {
+            constexpr bool W = decltype(w_c)::value;
+            if (u == 1) go(qk_rope_kernel<T, L, true, true, BWD, W, 1>);
+            else if (u == 2) go(qk_rope_kernel<T, L, true, true, BWD, W, 2>);
+            else if (u == 3) go(qk_rope_kernel<T, L, true, true, BWD, W, 3>);
+            else if constexpr (!BWD) go(qk_rope_kernel<T, L, true, true, BWD, W, 4>);
+        };
+        if (!aligned) go(qk_rope_kernel<T, L, false, false, BWD, true, 1>);
+        else if (!regular) go(qk_rope_kernel<T, L, true, false, BWD, true, 1>);
+        else if (weights) steps_of(std::true_type{});
+        else steps_of(std::false_type{});
     };
     switch (lpr) {
-        case 2: pick(std::integral_constant<int, 2>{}); break;
-        case 4: pick(std::integral_constant<int, 4>{}); break;
         case 8: pick(std::integral_constant<int, 8>{}); break;
         case 16: pick(std::integral_constant<int, 16>{}); break;
         case 32: pick(std::integral_constant<int, 32>{}); break;
         default: pick(std::integral_constant<int, 64>{}); break;
     }
-    *blocks = (int)grid;
+    *blocks = (int)(gx * gy);
     return check_launch("qk_rope_kernel");
 }
 
@@ -351,6 +374,8 @@ int rope_args(const char* who, RopeArgs& a, const void* q, const int64_t* qs, co
     if (B <= 0 || T <= 0 || Hq <= 0 || Hk <= 0 || P <= 0) return fail(NGPT_EINVAL, "%s: empty problem B=%d T=%d Hq=%d Hk=%d P=%d", who, B, T, Hq, Hk, P);
     if (D < 2 || D > 512) return fail(NGPT_ERANGE, "%s: head size %d outside 2 .. 512", who, D);
     if (R < 2 || R > D || R % 2) return fail(NGPT_EALIGN, "%s: %d rotated values of %d: need an even number from 2 to the head size", who, R, D);
+    if ((int64_t)B * T > (1 << 30)) return fail(NGPT_ERANGE, "%s: %lld tokens", who, (long long)B * T);
+    if (Hq > (1 << 20) || Hk > (1 << 20)) return fail(NGPT_ERANGE, "%s: Hq=%d Hk=%d", who, Hq, Hk);
     if (!pos && T > P) return fail(NGPT_ERANGE, "%s: %d positions in the tables, %d tokens in a sequence", who, P, T);
     if (pos && !ps) return fail(NGPT_EINVAL, "%s: positions without strides", who);
     if (!(eps >= 0.0f)) return fail(NGPT_ERANGE, "%s: eps=%g", who, (double)eps);
@@ -368,10 +393,10 @@ int rope_args(const char* who, RopeArgs& a, const void* q, const int64_t* qs, co
     return NGPT_OK;
 }
 
-// 16-byte accesses: every row starts on 16 bytes and the pairs' halves are whole 8-value pieces.
+// 16-byte accesses: every head starts on 16 bytes.
 bool rope_aligned(const RopeArgs& a, int dtype, bool bwd) {
     const int64_t per16 = dtype == NGPT_DT_BF16 ? 8 : 4;
-    bool ok = a.D % 8 == 0 && (a.interleaved ? a.R % 2 == 0 : a.R % 16 == 0) && aligned16(a.q) && aligned16(a.k) && aligned16(a.q_out) && aligned16(a.k_out);
+    bool ok = a.D % 8 == 0 && aligned16(a.q) && aligned16(a.k) && aligned16(a.q_out) && aligned16(a.k_out);
     for (int64_t s : {a.q_sb, a.q_st, a.q_sh, a.k_sb, a.k_st, a.k_sh}) ok = ok && s % per16 == 0;
     if (bwd) {
         ok = ok && aligned16(a.dq) && aligned16(a.dk);
@@ -379,6 +404,8 @@ bool rope_aligned(const RopeArgs& a, int dtype, bool bwd) {
     }
     return ok;
 }
+// Halves of whole 8-value pieces (pairs of neighbours: whole pieces), rows of the tables on 16 bytes.
+bool rope_regular(const RopeArgs& a) { return (a.interleaved ? a.R % 8 == 0 : a.R % 16 == 0) && aligned16(a.cos) && aligned16(a.sin); }
 
 }  // namespace
 }  // namespace ngpt
@@ -396,11 +423,11 @@ extern "C" int ngpt_qk_norm_rope(const void* q, const int64_t* q_strides, const 
     const bool al = rope_aligned(a, dtype, false);
     ProfileScope prof(PROF_PRODUCERS, (hipStream_t)stream);
     int blocks = 0;
-    return dtype == NGPT_DT_BF16 ? launch_rope<uint16_t, false>(a, al, &blocks, (hipStream_t)stream)
-                                 : launch_rope<float, false>(a, al, &blocks, (hipStream_t)stream);
+    return dtype == NGPT_DT_BF16 ? launch_rope<uint16_t, false>(a, al, rope_regular(a), &blocks, (hipStream_t)stream)
+                                 : launch_rope<float, false>(a, al, rope_regular(a), &blocks, (hipStream_t)stream);
 }
 
-extern "C" int64_t ngpt_qk_norm_rope_bwd_workspace_bytes(int D) { return (int64_t)kRopeMaxBlocks * 2 * (D > 0 ? D : 0) * 4; }
+extern "C" int64_t ngpt_qk_norm_rope_bwd_workspace_bytes(int D) { return (int64_t)kRopeSumBlocks * 2 * (D > 0 ? D : 0) * 4; }
 
 extern "C" int ngpt_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_strides, const void* dk_out, const int64_t* dk_strides,
                                      const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
@@ -427,10 +454,10 @@ extern "C" int ngpt_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_strid
     hipStream_t st = (hipStream_t)stream;
     ProfileScope prof(PROF_PRODUCERS, st);
     int blocks = 0;
-    if (int e = dtype == NGPT_DT_BF16 ? launch_rope<uint16_t, true>(a, al, &blocks, st) : launch_rope<float, true>(a, al, &blocks, st)) return e;
+    if (int e = dtype == NGPT_DT_BF16 ? launch_rope<uint16_t, true>(a, al, rope_regular(a), &blocks, st) : launch_rope<float, true>(a, al, rope_regular(a), &blocks, st)) return e;
     if (!want_dw) return NGPT_OK;
     const int grid = (2 * D + 31) / 32;
-    if (dtype == NGPT_DT_BF16) rope_dw_kernel<uint16_t><<<grid, 256, 0, st>>>(a.dw_part, blocks, D, (uint16_t*)dq_weight, (uint16_t*)dk_weight);
-    else rope_dw_kernel<float><<<grid, 256, 0, st>>>(a.dw_part, blocks, D, (float*)dq_weight, (float*)dk_weight);
+    if (dtype == NGPT_DT_BF16) rope_dw_kernel<uint16_t><<<grid, kColSumThreads, 0, st>>>(a.dw_part, blocks, D, (uint16_t*)dq_weight, (uint16_t*)dk_weight);
+    else rope_dw_kernel<float><<<grid, kColSumThreads, 0, st>>>(a.dw_part, blocks, D, (float*)dq_weight, (float*)dk_weight);
     return check_launch("rope_dw_kernel");
 }
