@@ -11,40 +11,62 @@ on one GPU; work is enqueued on that GPU's current stream.  There is no CPU impl
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
+import functools
 
 import torch
 from torch import Tensor
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .ops import _p, _stream, _workspace
+from .ops import _p, _workspace
+
+# the current stream's handle without the Stream object around it
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 ACTIVATIONS = {"none": 0, "relu2": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 RMS_EPS = 1.1920928955078125e-07          # machine epsilon of fp32, what the other norms of this package add
 _DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
 
 
-def _same_gpu(first: Tensor, *others: Tensor | None) -> None:
+def _same_gpu(first: Tensor, *others: Tensor | None) -> int:
+    """Index of the GPU that holds all of them."""
+    index = first.get_device()
     for t in (first, *others):
-        if t is not None and not t.is_cuda:
+        if t is not None and t.get_device() != index or index < 0:
+            if t is None or t.is_cuda and index >= 0:
+                raise AssertionError(f"tensors on {first.device} and {t.device}")
             raise RuntimeError("nanogpt operators run on the GPU only (got a CPU tensor); there is no CPU fallback")
-        assert t is None or t.device == first.device, f"tensors on {first.device} and {t.device}"
+    return index
 
 
-def _on(t: Tensor):
-    """Makes the tensor's GPU the current one for a launch."""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _launch(index: int, what: str, *args) -> None:
+    """Calls an entry point on GPU `index` and its current stream."""
+    fn = getattr(_lib.load(), what)
+    if index == torch.cuda.current_device():
+        code = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            code = fn(*args, _raw_stream(index))
+    if code:
+        _lib.check(code, what)
 
 
 def _plain(*tensors: Tensor | None) -> bool:
     """Ordinary tensors outside of a trace: the kernels can be launched here."""
-    return not torch.compiler.is_compiling() and all(t is None or type(t) in (Tensor, torch.nn.Parameter) for t in tensors)
+    for t in tensors:
+        if t is not None and type(t) is not Tensor and type(t) is not torch.nn.Parameter:
+            return False
+    return not torch.compiler.is_compiling()
 
 
 def _needs_grad(*tensors: Tensor | None) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 # ------------------------------------------------------------------------------------------------
@@ -81,7 +103,7 @@ def _rows(t: Tensor) -> Tensor:
 
 def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str, keep_pre: bool) -> tuple[Tensor, Tensor | None]:
     act = _linear_shapes(x, w, bias, residual, activation)
-    _same_gpu(x, w, bias, residual)
+    gpu = _same_gpu(x, w, bias, residual)
     N, K = w.shape
     out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
     pre = torch.empty_like(out) if keep_pre else None
@@ -94,11 +116,10 @@ def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | No
     res = None if residual is None else _matrix(residual)
     lib = _lib.load()
     M = xr.shape[0]
-    with _on(x):
-        nws = lib.ngpt_linear_act_fwd_workspace_bytes(M, N, K)
-        ws = _workspace(nws, x.device) if nws else None
-        _lib.check(lib.ngpt_linear_act_fwd(_p(xr), _ld(xr), _p(wr), _ld(wr), _p(bias), _p(res), 0 if res is None else _ld(res),
-                                           M, N, K, act, _p(out), _p(pre), _p(ws), nws, _stream(x)), "ngpt_linear_act_fwd")
+    nws = lib.ngpt_linear_act_fwd_workspace_bytes(M, N, K)
+    ws = _workspace(nws, x.device) if nws else None
+    _launch(gpu, "ngpt_linear_act_fwd", _p(xr), _ld(xr), _p(wr), _ld(wr), _p(bias), _p(res), 0 if res is None else _ld(res), M, N, K, act,
+            _p(out), _p(pre), _p(ws), nws)
     return out, pre
 
 
@@ -107,7 +128,7 @@ def _linear_bwd(dout: Tensor, x: Tensor, w: Tensor, pre: Tensor | None, activati
     act = ACTIVATIONS[activation]
     assert dout.shape == (*x.shape[:-1], w.shape[0]) and dout.dtype == torch.bfloat16
     assert act == 0 or pre is not None, "the backward of an activation needs the forward's pre-activation"
-    _same_gpu(x, w, dout, pre)
+    gpu = _same_gpu(x, w, dout, pre)
     N, K = w.shape
     new = lambda *shape: torch.empty(shape, dtype=torch.bfloat16, device=x.device)
     dx = new(*x.shape) if need_dx else None
@@ -124,11 +145,8 @@ def _linear_bwd(dout: Tensor, x: Tensor, w: Tensor, pre: Tensor | None, activati
     dout = dout.contiguous()
     pre = None if pre is None else pre.contiguous()
     xr, wr = _rows(x), _rows(w)
-    lib = _lib.load()
-    with _on(x):
-        ws = _workspace(lib.ngpt_linear_act_bwd_workspace_bytes(M, N, K), x.device)
-        _lib.check(lib.ngpt_linear_act_bwd(_p(dout), _p(pre), _p(xr), _ld(xr), _p(wr), _ld(wr), M, N, K, act,
-                                           _p(dx), _p(dw), _p(db), _p(ws), ws.numel(), _stream(x)), "ngpt_linear_act_bwd")
+    ws = _workspace(_lib.load().ngpt_linear_act_bwd_workspace_bytes(M, N, K), x.device)
+    _launch(gpu, "ngpt_linear_act_bwd", _p(dout), _p(pre), _p(xr), _ld(xr), _p(wr), _ld(wr), M, N, K, act, _p(dx), _p(dw), _p(db), _p(ws), ws.numel())
     return dx, dw, db
 
 
@@ -229,7 +247,9 @@ def _heads(t: Tensor) -> Tensor:
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+@functools.lru_cache(maxsize=1024)
 def _strides(*s: int):
+    """The strides as a C array (read only, so one per value will do)."""
     return (ctypes.c_int64 * len(s))(*s)
 
 
@@ -257,22 +277,20 @@ def _rope_common(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved
 
 def _rope_fwd(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved) -> tuple[Tensor, Tensor]:
     _rope_shapes(q, k, cos, sin, positions, q_weight, k_weight)
-    _same_gpu(q, k, cos, sin, positions, q_weight, k_weight)
+    gpu = _same_gpu(q, k, cos, sin, positions, q_weight, k_weight)
     q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
     if q.numel() == 0 and k.numel() == 0:
         return q_out, k_out
     q, k = _heads(q), _heads(k)
     keep, args = _rope_common(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
-    with _on(q):
-        _lib.check(_lib.load().ngpt_qk_norm_rope(_p(q), _head_strides(q), _p(k), _head_strides(k), *args, _p(q_out), _p(k_out), _stream(q)),
-                   "ngpt_qk_norm_rope")
+    _launch(gpu, "ngpt_qk_norm_rope", _p(q), _head_strides(q), _p(k), _head_strides(k), *args, _p(q_out), _p(k_out))
     return q_out, k_out
 
 
 def _rope_bwd(dq_out, dk_out, q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved, need_dqw, need_dkw):
     """-> dq, dk, dq_weight or None, dk_weight or None"""
-    _same_gpu(q, k, cos, sin, positions, q_weight, k_weight, dq_out, dk_out)
+    gpu = _same_gpu(q, k, cos, sin, positions, q_weight, k_weight, dq_out, dk_out)
     assert dq_out.shape == q.shape and dk_out.shape == k.shape and dq_out.dtype == q.dtype and dk_out.dtype == k.dtype
     dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
     dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
@@ -285,13 +303,10 @@ def _rope_bwd(dq_out, dk_out, q, k, cos, sin, positions, q_weight, k_weight, eps
         return dq, dk, dqw, dkw
     q, k, dq_out, dk_out = _heads(q), _heads(k), _heads(dq_out), _heads(dk_out)
     keep, args = _rope_common(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved)
-    lib = _lib.load()
-    with _on(q):
-        nws = lib.ngpt_qk_norm_rope_bwd_workspace_bytes(q.shape[-1]) if need_dqw or need_dkw else 0
-        ws = _workspace(nws, q.device) if nws else None
-        _lib.check(lib.ngpt_qk_norm_rope_bwd(_p(dq_out), _head_strides(dq_out), _p(dk_out), _head_strides(dk_out), _p(q), _head_strides(q), _p(k),
-                                             _head_strides(k), *args, _p(dq), _p(dk), _p(dqw), _p(dkw), _p(ws), nws, _stream(q)),
-                   "ngpt_qk_norm_rope_bwd")
+    nws = _lib.load().ngpt_qk_norm_rope_bwd_workspace_bytes(q.shape[-1]) if need_dqw or need_dkw else 0
+    ws = _workspace(nws, q.device) if nws else None
+    _launch(gpu, "ngpt_qk_norm_rope_bwd", _p(dq_out), _head_strides(dq_out), _p(dk_out), _head_strides(dk_out), _p(q), _head_strides(q), _p(k),
+            _head_strides(k), *args, _p(dq), _p(dk), _p(dqw), _p(dkw), _p(ws), nws)
     return dq, dk, dqw, dkw
 
 
@@ -384,39 +399,36 @@ def _distill_shapes(logits, ids, teacher, teacher_lse, row_weight) -> None:
 
 def _distill_args(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C):
     _distill_shapes(logits, ids, teacher, teacher_lse, row_weight)
-    _same_gpu(logits, ids, teacher, teacher_lse, row_weight)
+    gpu = _same_gpu(logits, ids, teacher, teacher_lse, row_weight)
     keep = [_matrix(logits)] + [None if t is None else t.contiguous() for t in (ids, teacher, teacher_lse, row_weight)]
     lg, i, t, l, w = keep
     T, V = lg.shape
-    return keep, (_p(lg), _DTYPES[lg.dtype], _ld(lg), _p(i), int(i.dtype == torch.int64), _p(t), _p(l), _p(w), T, V, i.shape[1],
+    return gpu, keep, (_p(lg), _DTYPES[lg.dtype], _ld(lg), _p(i), int(i.dtype == torch.int64), _p(t), _p(l), _p(w), T, V, i.shape[1],
                   temperature, A, B, C)
 
 
 def _distill_fwd(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C, keep_stats: bool) -> tuple[Tensor, Tensor | None]:
-    keep, args = _distill_args(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C)
+    gpu, keep, args = _distill_args(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C)
     losses = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
     stats = torch.empty((logits.shape[0], 4), dtype=torch.float32, device=logits.device) if keep_stats else None
     if losses.numel() == 0:
         return losses, stats
     if ids.shape[1] == 0:
         return losses.zero_(), None if stats is None else stats.zero_()
-    with _on(logits):
-        _lib.check(_lib.load().ngpt_distill_fwd(*args, _p(losses), _p(stats), _stream(logits)), "ngpt_distill_fwd")
+    _launch(gpu, "ngpt_distill_fwd", *args, _p(losses), _p(stats))
     return losses, stats
 
 
 def _distill_bwd(dlosses, logits, ids, teacher, teacher_lse, row_weight, stats, temperature, A, B, C) -> Tensor:
     assert dlosses.shape == (logits.shape[0],) and dlosses.dtype == torch.float32
     _same_gpu(logits, dlosses, stats)
-    keep, args = _distill_args(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C)
+    gpu, keep, args = _distill_args(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
     if grad.numel() == 0:
         return grad
     if ids.shape[1] == 0:
         return grad.zero_()
-    with _on(logits):
-        _lib.check(_lib.load().ngpt_distill_bwd(*args, _p(stats), _p(dlosses), dlosses.stride(0), _p(grad), _ld(grad), _stream(logits)),
-                   "ngpt_distill_bwd")
+    _launch(gpu, "ngpt_distill_bwd", *args, _p(stats), _p(dlosses), dlosses.stride(0), _p(grad), _ld(grad))
     return grad
 
 
@@ -427,11 +439,10 @@ def _distill_fused(logits, ids, teacher, teacher_lse, row_weight, temperature, A
         losses, stats = _distill_fwd(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C, True)
         scale = torch.full((1,), grad_scale, dtype=torch.float32, device=logits.device).expand(logits.shape[0])
         return losses, _distill_bwd(scale, logits, ids, teacher, teacher_lse, row_weight, stats, temperature, A, B, C)
-    keep, args = _distill_args(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C)
+    gpu, keep, args = _distill_args(logits, ids, teacher, teacher_lse, row_weight, temperature, A, B, C)
     losses = torch.empty(logits.shape[0], dtype=torch.float32, device=logits.device)
     grad = torch.empty(logits.shape, dtype=logits.dtype, device=logits.device)
-    with _on(logits):
-        _lib.check(lib.ngpt_distill_fwd_bwd(*args, grad_scale, _p(losses), _p(grad), _ld(grad), _stream(logits)), "ngpt_distill_fwd_bwd")
+    _launch(gpu, "ngpt_distill_fwd_bwd", *args, grad_scale, _p(losses), _p(grad), _ld(grad))
     return losses, grad
 
 
