@@ -340,8 +340,10 @@ int ngpt_lmhead_ce_bwd_codes(const void* x_f8, const void* w_f8_vk, const int64_
 
 /* ---- matrix product with bias, activation and residual in its epilogue ---------------------------
  * out [M, N] = residual + act(x [M, K] . w [N, K]^T + bias [N]), bf16 in and out, fp32 in between, rounded once.  bias and residual are nullable.
+ * The bias starts on 16 bytes.
  * Row strides in elements; where K % 64 == 0 rows of x and w must start on 16 bytes (otherwise both are copied into the workspace).
- * Any M, N, K.  pre [M, N] (nullable) receives bf16(x w^T + bias), what the backward of an activation needs. */
+ * Any M, N, K.  pre [M, N] (nullable; null for NGPT_ACT_NONE) receives bf16(x w^T + bias), what the backward of an
+ * activation needs. */
 int64_t ngpt_linear_act_fwd_workspace_bytes(int M, int N, int K);
 int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw, const void* bias_bf16,
                         const void* residual_bf16, int64_t ld_residual, int M, int N, int K, int activation,

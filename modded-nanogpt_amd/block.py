@@ -103,6 +103,7 @@ def _rows(t: Tensor) -> Tensor:
 
 def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str, keep_pre: bool) -> tuple[Tensor, Tensor | None]:
     act = _linear_shapes(x, w, bias, residual, activation)
+    assert act or not keep_pre, "keep_pre: without an activation the backward needs no pre-activation"
     gpu = _same_gpu(x, w, bias, residual)
     N, K = w.shape
     out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
@@ -112,7 +113,8 @@ def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | No
     if K == 0:
         raise RuntimeError("linear_act: contraction of length 0")
     xr, wr = _rows(x), _rows(w)
-    bias = None if bias is None else bias.contiguous()
+    if bias is not None and (bias.stride(0) != 1 or bias.data_ptr() % 16):
+        bias = bias.clone(memory_format=torch.contiguous_format)
     res = None if residual is None else _matrix(residual)
     lib = _lib.load()
     M = xr.shape[0]

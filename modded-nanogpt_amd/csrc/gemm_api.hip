@@ -119,8 +119,7 @@ static BalancePlan plan_balance(int R, int C, int K) {
 // Adds up the parts of the split tiles and writes them out.  Tile number first + blockIdx.x of the walk order is the
 // blockIdx.x-th split tile; its `splits` parts are the fp32 tiles number s * gridDim.x + blockIdx.x of `part32`
 // (GridIter::part_slot), summed in the order of the contraction.  T = uint16_t: bf16 output, T = float: fp32.
-constexpr int kRemSlices = 8;
-static_assert(MainCfg::BM % kRemSlices == 0, "row slices of a tile");
+static_assert(MainCfg::BM % 32 == 0, "row slices of a tile");
 template <class T>
 __global__ __launch_bounds__(256) void rem_tiles_kernel(const float* __restrict__ part32, int splits, T* __restrict__ out, int64_t ldo,
                                                         int R, int C, int first) {
@@ -128,7 +127,8 @@ __global__ __launch_bounds__(256) void rem_tiles_kernel(const float* __restrict_
     int tr, tc;
     order.coords(first + blockIdx.x, tr, tc);
     // blockIdx.y: which slice of the tile's rows (a few dozen tiles alone would leave most of the chip idle)
-    constexpr int rows = MainCfg::BM / kRemSlices, cols4 = MainCfg::BN / 4, tile_elems = MainCfg::BM * MainCfg::BN;
+    const int rows = MainCfg::BM / gridDim.y;
+    constexpr int cols4 = MainCfg::BN / 4, tile_elems = MainCfg::BM * MainCfg::BN;
     const int rl0 = blockIdx.y * rows;
     const int64_t part_stride = (int64_t)gridDim.x * tile_elems;
     for (int i = threadIdx.x; i < rows * cols4; i += blockDim.x) {
@@ -137,11 +137,23 @@ __global__ __launch_bounds__(256) void rem_tiles_kernel(const float* __restrict_
         if (r >= R || c >= C) continue;          // C % 4 == 0 is checked by the caller
         const float* p = part32 + (int64_t)blockIdx.x * tile_elems + rl * MainCfg::BN + cl;
         v4f v = *(const v4f*)p;
-        for (int s_ = 1; s_ < splits; ++s_) v += *(const v4f*)(p + s_ * part_stride);
+        int s_ = 1;
+        for (; s_ + 4 <= splits; s_ += 4) {      // four loads in flight, added in order
+            const v4f a0 = *(const v4f*)(p + s_ * part_stride), a1 = *(const v4f*)(p + (s_ + 1) * part_stride);
+            const v4f a2 = *(const v4f*)(p + (s_ + 2) * part_stride), a3 = *(const v4f*)(p + (s_ + 3) * part_stride);
+            v += a0;
+            v += a1;
+            v += a2;
+            v += a3;
+        }
+        for (; s_ < splits; ++s_) v += *(const v4f*)(p + s_ * part_stride);
         if constexpr (sizeof(T) == 2) *(v2i*)(out + (int64_t)r * ldo + c) = (v2i){(int)cvt_pk_bf16(v[0], v[1]), (int)cvt_pk_bf16(v[2], v[3])};
         else *(v4f*)(out + (int64_t)r * ldo + c) = v;
     }
 }
+
+// Row slices a summed tile is cut into: 8 where the tiles alone keep half the chip busy that way, else 32.
+static int rem_slices(int tiles) { return 2 * 8 * tiles > num_cus() ? 8 : 32; }
 
 // Bytes of fp32 scratch a balanced GEMM may need for the parts of its split tiles, whatever the device: at most one
 // part per workgroup of the last round (kMaxGrid bounds the grid) and never more than tiles x splits.
@@ -169,7 +181,7 @@ int gemm_balanced_bf16(const void* A, int fa, int64_t lda, const void* B, int fb
     GemmOperands g{(const uint8_t*)A, (const uint8_t*)B, lda, ldb, R, C, K, p.splits, layout, p.full, a_rows_pad};
     EpiStoreBf16 epi{(uint16_t*)out_bf16, ldc, scale, R, C, part32, false, 0, dscale_a, dscale_b};
     if (int e = launch_gemm<MainCfg>(g, fa, fb, epi, st)) return e;
-    if (p.splits > 1) rem_tiles_kernel<uint16_t><<<dim3(p.rem, kRemSlices), 256, 0, st>>>(part32, p.splits, (uint16_t*)out_bf16, ldc, R, C, p.full);
+    if (p.splits > 1) rem_tiles_kernel<uint16_t><<<dim3(p.rem, rem_slices(p.rem)), 256, 0, st>>>(part32, p.splits, (uint16_t*)out_bf16, ldc, R, C, p.full);
     return check_launch("gemm_balanced_bf16");
 }
 
@@ -186,7 +198,7 @@ int gemm_bf16_clipped(const void* A, int fa, int64_t lda, const void* B, int fb,
     GemmOperands g{(const uint8_t*)A, (const uint8_t*)B, lda, ldb, R, C, K, p.splits, 0, p.full, 0};
     EpiStoreBf16 epi{(uint16_t*)out_bf16, ldc, 1.0f, R_out, C_out, part32, false, 0, nullptr, nullptr};
     if (int e = launch_gemm<MainCfg>(g, fa, fb, epi, st)) return e;
-    if (p.splits > 1) rem_tiles_kernel<uint16_t><<<dim3(p.rem, kRemSlices), 256, 0, st>>>(part32, p.splits, (uint16_t*)out_bf16, ldc, R_out, C_out, p.full);
+    if (p.splits > 1) rem_tiles_kernel<uint16_t><<<dim3(p.rem, rem_slices(p.rem)), 256, 0, st>>>(part32, p.splits, (uint16_t*)out_bf16, ldc, R_out, C_out, p.full);
     return check_launch("gemm_bf16_clipped");
 }
 
@@ -206,7 +218,7 @@ int gemm_balanced_f32(const void* A, int fa, int64_t lda, const void* B, int fb,
     if (p.splits > 1 && (!part32 || p.rem * p.splits > kMaxGrid)) return fail(NGPT_EINVAL, "gemm_balanced_f32: split tiles need the fp32 scratch tiles");
     EpiStoreF32<false> epi{out, ldc, scale, R, C, part32, false, 0};
     if (int e = launch_gemm<MainCfg>(g, fa, fb, epi, st)) return e;
-    if (p.splits > 1) rem_tiles_kernel<float><<<dim3(p.rem, kRemSlices), 256, 0, st>>>(part32, p.splits, out, ldc, R, C, p.full);
+    if (p.splits > 1) rem_tiles_kernel<float><<<dim3(p.rem, rem_slices(p.rem)), 256, 0, st>>>(part32, p.splits, out, ldc, R, C, p.full);
     return check_launch("gemm_balanced_f32");
 }
 

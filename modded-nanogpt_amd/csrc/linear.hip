@@ -53,18 +53,7 @@ __device__ __forceinline__ float act_slope(float z) {
         return 1.0f;
     }
 }
-// f(integral_constant) for the activation, a wave-uniform branch
-template <class F>
-__device__ __forceinline__ void with_act(int act, F&& f) {
-    switch (act) {
-        case NGPT_ACT_RELU2: f(std::integral_constant<int, NGPT_ACT_RELU2>{}); break;
-        case NGPT_ACT_GELU: f(std::integral_constant<int, NGPT_ACT_GELU>{}); break;
-        case NGPT_ACT_GELU_TANH: f(std::integral_constant<int, NGPT_ACT_GELU_TANH>{}); break;
-        case NGPT_ACT_SILU: f(std::integral_constant<int, NGPT_ACT_SILU>{}); break;
-        default: break;
-    }
-}
-
+typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float lo16(int w) { return __uint_as_float((uint32_t)w << 16); }
 __device__ __forceinline__ float hi16(int w) { return __uint_as_float((uint32_t)w & 0xffff0000u); }
 
@@ -102,22 +91,29 @@ __device__ __forceinline__ void store8(uint16_t* p, v4i w, int n, bool vec) {
 // x and four consecutive features per accumulator register group.  Every 32-row x 64-feature block passes through the wave's 4 KiB
 // of LDS, so that z, the residual and the output cross memory as whole 128-byte lines.  16-byte pieces are XOR-swizzled by
 // the row; LDS operations of one wave execute in order, no waits are needed between the steps.
-template <int WAVES, bool PRE>
+// Memory is reached through descriptors of the tile's rows, whose bounds check stands for the branches at the matrix' end: a kernel of
+// many basic blocks is not inlined completely any more, and the GEMM's state then lives in scratch memory.  Rows that do not start on
+// 16 bytes are moved value by value, in loops.
+__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, int64_t bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)(bytes < 0x7fffff00 ? bytes : 0x7fffff00), 0x00020000);
+}
+constexpr int kNowhere = 0x7ffffff0;      // an offset past any descriptor's end
+
+// One kernel an activation: five of them behind a switch in one kernel cost it 60 spilled registers.
+template <int WAVES, int ACT, bool PRE, bool RES>
 struct EpiLinear {
     uint16_t* out;          // [C, R], row stride R
     uint16_t* pre;          // PRE: z, same shape
-    const uint16_t* bias;   // nullable [R]
-    const uint16_t* res;    // nullable [C, R], row stride ld_res
+    const uint16_t* bias;   // nullable [R], on 16 bytes
+    const uint16_t* res;    // RES: [C, R], row stride ld_res
     int64_t ld_res;
-    int act;
     int R, C;
-    int vec, vec_res;       // rows of out and pre / of res start on 16 bytes
-    int vec_bias;           // bias starts on 8 bytes
+    int vec, vec_res;       // rows of out and pre / of res start on 16 bytes and are whole 8-value pieces
     static constexpr int EXTRA_LDS = WAVES * 4096;
     static constexpr bool NEEDS_SCRATCH = false;
     static constexpr bool JOB_END_NEEDS_SCRATCH = false;
     static constexpr bool DROPS_FRAGMENTS = true;   // the residual's lines in flight next to the accumulators
-    static constexpr int TILE_STORES = 16;          // at least (4 per 32-row block and wave), in a tile that lies inside the matrix
+    static constexpr int TILE_STORES = 8;           // at least: 4 per 32-row block and wave, 2 blocks or more (masked ones are issued too)
     uint8_t* stage;
     bool stored_all;
     __device__ bool all_stores_issued() const { return stored_all; }
@@ -131,108 +127,113 @@ struct EpiLinear {
     __device__ void job_begin(int) {}
     template <class Cfg>
     __device__ void job_end(int, int, const AccCoords<Cfg>&, uint8_t*) {}
-    template <class Cfg>
-    __device__ __forceinline__ void tile(v16f (&acc)[Cfg::TM][Cfg::TN], int r0, int c0, const AccCoords<Cfg>& co, uint8_t*, int lane) {
-        static_assert(Cfg::TM == 2 && Cfg::NWAVES == WAVES, "64-feature wave tiles, 4 KiB of staging each");
-        const int h = lane >> 5, j = lane & 31;
-        const bool full = (r0 + Cfg::BM <= R) && (c0 + Cfg::BN <= C);
-        stored_all = full && vec && Cfg::TN >= 4;
-        const int rd_row = lane >> 3, rd_chunk = lane & 7;
-        const int f = r0 + co.wave_row0 + rd_chunk * 8;          // this lane's 8 features in the line-wise steps
-        const int left = R - f;
-        v2i b[8];                                                // bias of the lane's features, packed
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = r0 + co.wave_row0 + 8 * i + 4 * h;
-            b[i] = (v2i){0, 0};
-            if (bias) {
-                if (vec_bias && c + 4 <= R) {
-                    b[i] = *(const v2i*)(bias + c);
-                } else {
+
+    // the wave's block of 32 rows x 64 features, `row0` / `col0` its origin in the matrix, value by value
+    __device__ __forceinline__ void block_slow(const uint16_t* from, uint16_t* to, int64_t ld, int row0, int col0, int lane) {
 #pragma unroll 1
-                    for (int e = min(4, R - c) - 1; e >= 0; --e) {
-                        b[i].y = (int)__builtin_amdgcn_alignbit((uint32_t)b[i].y, (uint32_t)b[i].x, 16);
-                        b[i].x = (int)(((uint32_t)b[i].x << 16) | (uint32_t)bias[c + e]);
-                    }
-                }
+        for (int i = 0; i < 32; ++i) {
+            const int m = row0 + i, f = col0 + lane;
+            uint16_t* at = (uint16_t*)(stage + i * 128 + (((lane >> 3) ^ (i & 7)) << 4) + (lane & 7) * 2);
+            if (m < C && f < R) {
+                if (to) to[(int64_t)m * ld + f] = *at;
+                else *at = from[(int64_t)m * ld + f];
             }
         }
-        const bool has_res = res != nullptr;
-        v4i line[Cfg::TN][4];
+    }
+
+    template <class Cfg>
+    __device__ __forceinline__ void tile(v16f (&acc)[Cfg::TM][Cfg::TN], int r0, int c0, const AccCoords<Cfg>& co, uint8_t*, int lane) {
+        static_assert(Cfg::TM == 2 && Cfg::TN >= 2 && Cfg::NWAVES == WAVES, "64-feature wave tiles, 4 KiB of staging each");
+        const int h = lane >> 5, j = lane & 31;
+        stored_all = vec != 0;
+        const int rd_row = lane >> 3, rd_chunk = lane & 7;
+        const int f = r0 + co.wave_row0 + rd_chunk * 8;          // this lane's 8 features in the line-wise steps
+        const int rows = C - c0;                                 // rows of the matrix from this tile on
+        const bool in = f < R;                                   // (R is a multiple of 8 where whole lines are moved)
+        const auto buf_out = buffer_of(out + (int64_t)c0 * R, (int64_t)rows * R * 2);
+        const auto buf_pre = buffer_of(PRE ? pre + (int64_t)c0 * R : out, PRE ? (int64_t)rows * R * 2 : 0);
+        const auto buf_res = buffer_of(RES ? res + (int64_t)c0 * ld_res : out, RES ? ((int64_t)(rows - 1) * ld_res + R) * 2 : 0);
+        const auto buf_bias = buffer_of(bias, bias ? ((int64_t)R * 2 + 3) & ~3ll : 0);
+        const int off = in ? ((co.wave_col0 + rd_row) * R + f) * 2 : kNowhere;
+        const int off_res = RES && in ? (int)(((co.wave_col0 + rd_row) * ld_res + f) * 2) : kNowhere;
+        v2i b[8];                                                // bias of the lane's features, packed
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            b[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(buf_bias, (r0 + co.wave_row0 + 8 * i + 4 * h) * 2, 0, 0));
+        v4i line[4];
         auto load_block = [&](int tn) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int m = c0 + co.wave_col0 + tn * 32 + 8 * k + rd_row;
-                line[tn][k] = m < C ? load8(res + (int64_t)m * ld_res + f, left, vec_res != 0) : (v4i){0, 0, 0, 0};
-            }
+            for (int k = 0; k < 4; ++k)
+                line[k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(buf_res, in ? off_res + (int)((tn * 32 + 8 * k) * ld_res * 2) : kNowhere, 0, 0));
         };
-        auto store_block = [&](int tn, uint16_t* to) {
+        auto store_block = [&](int tn, __amdgpu_buffer_rsrc_t buf, uint16_t* to) {
+            if (vec) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int row = 8 * k + rd_row;
-                const v4i v = *(const v4i*)(stage + row * 128 + ((rd_chunk ^ (row & 7)) << 4));
-                const int m = c0 + co.wave_col0 + tn * 32 + row;
-                if (m < C) store8(to + (int64_t)m * R + f, v, left, vec != 0);
+                for (int k = 0; k < 4; ++k) {
+                    const int row = 8 * k + rd_row;
+                    const v4i v = *(const v4i*)(stage + row * 128 + ((rd_chunk ^ (row & 7)) << 4));
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), buf, in ? off + (tn * 32 + 8 * k) * R * 2 : kNowhere, 0, 0);
+                }
+            } else {
+                block_slow(nullptr, to, R, c0 + co.wave_col0 + tn * 32, r0 + co.wave_row0, lane);
             }
         };
-        if (has_res) load_block(0);
+        if constexpr (RES) { if (vec_res) load_block(0); }
 #pragma unroll
         for (int tn = 0; tn < Cfg::TN; ++tn) {
-            if (has_res && tn + 1 < Cfg::TN) load_block(tn + 1);
-            float z[2][16];
-#pragma unroll
-            for (int tm = 0; tm < 2; ++tm)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    z[tm][4 * g] = acc[tm][tn][4 * g] + lo16(b[tm * 4 + g].x);
-                    z[tm][4 * g + 1] = acc[tm][tn][4 * g + 1] + hi16(b[tm * 4 + g].x);
-                    z[tm][4 * g + 2] = acc[tm][tn][4 * g + 2] + lo16(b[tm * 4 + g].y);
-                    z[tm][4 * g + 3] = acc[tm][tn][4 * g + 3] + hi16(b[tm * 4 + g].y);
-                }
+            const v16f* const a2[2] = {&acc[0][tn], &acc[1][tn]};
+            auto z_of = [&](int tm, int g, float (&z)[4]) {
+                const v16f& a = *a2[tm];
+                const v2i bb = b[tm * 4 + g];
+                z[0] = a[4 * g] + lo16(bb.x);
+                z[1] = a[4 * g + 1] + hi16(bb.x);
+                z[2] = a[4 * g + 2] + lo16(bb.y);
+                z[3] = a[4 * g + 3] + hi16(bb.y);
+            };
+            auto place = [&](int tm, int g) { return stage + j * 128 + (((tm * 4 + g) ^ (j & 7)) << 4) + 8 * h; };
             if constexpr (PRE) {
 #pragma unroll
                 for (int tm = 0; tm < 2; ++tm)
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const float* a = z[tm];
-                        *(v2i*)(stage + j * 128 + (((tm * 4 + g) ^ (j & 7)) << 4) + 8 * h) =
-                            (v2i){(int)cvt_pk_bf16(a[4 * g], a[4 * g + 1]), (int)cvt_pk_bf16(a[4 * g + 2], a[4 * g + 3])};
+                        float z[4];
+                        z_of(tm, g, z);
+                        *(v2i*)place(tm, g) = (v2i){(int)cvt_pk_bf16(z[0], z[1]), (int)cvt_pk_bf16(z[2], z[3])};
                     }
-                store_block(tn, pre);
+                store_block(tn, buf_pre, pre);
             }
-            if (has_res) {
+            if constexpr (RES) {
+                if (vec_res) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = 8 * k + rd_row;
-                    *(v4i*)(stage + row * 128 + ((rd_chunk ^ (row & 7)) << 4)) = line[tn][k];
+                    for (int k = 0; k < 4; ++k) {
+                        const int row = 8 * k + rd_row;
+                        *(v4i*)(stage + row * 128 + ((rd_chunk ^ (row & 7)) << 4)) = line[k];
+                    }
+                    if (tn + 1 < Cfg::TN) load_block(tn + 1);       // in flight while this block is worked on
+                } else {
+                    block_slow(res, nullptr, ld_res, c0 + co.wave_col0 + tn * 32, r0 + co.wave_row0, lane);
                 }
             }
-            with_act(act, [&](auto kind) {
-#pragma unroll
-                for (int tm = 0; tm < 2; ++tm)
-#pragma unroll
-                    for (int v = 0; v < 16; ++v) {
-                        z[tm][v] = act_of<decltype(kind)::value>(z[tm][v]);
-                        if ((v & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // four at a time: few temporaries next to the accumulators
-                    }
-            });
 #pragma unroll
             for (int tm = 0; tm < 2; ++tm)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    uint8_t* at = stage + j * 128 + (((tm * 4 + g) ^ (j & 7)) << 4) + 8 * h;
-                    const float* a = z[tm];
-                    float y0 = a[4 * g], y1 = a[4 * g + 1], y2 = a[4 * g + 2], y3 = a[4 * g + 3];
-                    if (has_res) {
+                    uint8_t* at = place(tm, g);
+                    float z[4];
+                    z_of(tm, g, z);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) z[i] = act_of<ACT>(z[i]);
+                    if constexpr (RES) {
                         const v2i r = *(const v2i*)at;
-                        y0 += lo16(r.x);
-                        y1 += hi16(r.x);
-                        y2 += lo16(r.y);
-                        y3 += hi16(r.y);
+                        z[0] += lo16(r.x);
+                        z[1] += hi16(r.x);
+                        z[2] += lo16(r.y);
+                        z[3] += hi16(r.y);
                     }
-                    *(v2i*)at = (v2i){(int)cvt_pk_bf16(y0, y1), (int)cvt_pk_bf16(y2, y3)};
+                    *(v2i*)at = (v2i){(int)cvt_pk_bf16(z[0], z[1]), (int)cvt_pk_bf16(z[2], z[3])};
+                    if (g & 1) __builtin_amdgcn_sched_barrier(0);   // few temporaries next to the accumulators
                 }
-            store_block(tn, out);
+            store_block(tn, buf_out, out);
             __builtin_amdgcn_sched_barrier(0);
         }
     }
@@ -329,6 +330,18 @@ int act_grad_rows(int64_t M, int64_t N) {
     return (int)std::max<int64_t>(rows, 1);
 }
 
+// f(integral_constant) for the activation
+template <class F>
+auto with_act(int act, F&& f) {
+    switch (act) {
+        case NGPT_ACT_RELU2: return f(std::integral_constant<int, NGPT_ACT_RELU2>{});
+        case NGPT_ACT_GELU: return f(std::integral_constant<int, NGPT_ACT_GELU>{});
+        case NGPT_ACT_GELU_TANH: return f(std::integral_constant<int, NGPT_ACT_GELU_TANH>{});
+        case NGPT_ACT_SILU: return f(std::integral_constant<int, NGPT_ACT_SILU>{});
+        default: return f(std::integral_constant<int, NGPT_ACT_NONE>{});
+    }
+}
+
 int check_linear(const char* who, int M, int N, int K, int act) {
     if (M <= 0 || N <= 0 || K <= 0) return fail(NGPT_EINVAL, "%s: empty problem M=%d N=%d K=%d", who, M, N, K);
     if (act < NGPT_ACT_NONE || act > NGPT_ACT_SILU) return fail(NGPT_EINVAL, "%s: activation=%d", who, act);
@@ -355,6 +368,8 @@ extern "C" int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* 
     const char* who = "ngpt_linear_act_fwd";
     if (!x_bf16 || !w_bf16 || !out_bf16) return fail(NGPT_EINVAL, "%s: null pointer", who);
     if (int e = check_linear(who, M, N, K, activation)) return e;
+    if (pre_bf16 && activation == NGPT_ACT_NONE) return fail(NGPT_EINVAL, "%s: pre is for activations", who);
+    if (!on16(bias_bf16)) return fail(NGPT_EALIGN, "%s: the bias starts on 16 bytes", who);
     if (ldx < K || ldw < K || (residual_bf16 && ld_residual < N))
         return fail(NGPT_EALIGN, "%s: row strides ldx=%lld ldw=%lld ld_residual=%lld", who, (long long)ldx, (long long)ldw, (long long)ld_residual);
     hipStream_t st = (hipStream_t)stream;
@@ -381,18 +396,24 @@ extern "C" int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* 
         epi.bias = (const uint16_t*)bias_bf16;
         epi.res = (const uint16_t*)residual_bf16;
         epi.ld_res = ld_residual;
-        epi.act = activation;
         epi.R = N;
         epi.C = M;
         epi.vec = N % 8 == 0 && on16(out_bf16) && on16(pre_bf16);
-        epi.vec_bias = ((uintptr_t)bias_bf16 & 7) == 0;
-        epi.vec_res = residual_bf16 && ld_residual % 8 == 0 && on16(residual_bf16);
+        epi.vec_res = residual_bf16 && N % 8 == 0 && ld_residual % 8 == 0 && on16(residual_bf16);
         using Cfg = std::conditional_t<Epi::EXTRA_LDS == 8 * 4096, MainCfg, SmallCfg>;
         return launch_gemm_fmt<Cfg, FMT_BF16, FMT_BF16>(g, epi, st, 0);
     };
     const int64_t tiles = ((int64_t)(N + 255) / 256) * ((M + 255) / 256);
-    if (2 * tiles > num_cus()) return pre_bf16 ? go(EpiLinear<8, true>{}) : go(EpiLinear<8, false>{});
-    return pre_bf16 ? go(EpiLinear<4, true>{}) : go(EpiLinear<4, false>{});
+    auto pick = [&](auto waves, auto kind) {
+        constexpr int W = decltype(waves)::value, A = decltype(kind)::value;
+        if constexpr (A != NGPT_ACT_NONE) {
+            if (pre_bf16) return residual_bf16 ? go(EpiLinear<W, A, true, true>{}) : go(EpiLinear<W, A, true, false>{});
+        }
+        return residual_bf16 ? go(EpiLinear<W, A, false, true>{}) : go(EpiLinear<W, A, false, false>{});
+    };
+    return with_act(activation, [&](auto kind) {
+        return 2 * tiles > num_cus() ? pick(std::integral_constant<int, 8>{}, kind) : pick(std::integral_constant<int, 4>{}, kind);
+    });
 }
 
 namespace ngpt {
@@ -447,13 +468,7 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
             act_grad_kernel<decltype(kind)::value><<<grid, 256, 0, st>>>((const uint16_t*)dout_bf16, (const uint16_t*)pre_bf16, M, N,
                                                                          own_dz ? (uint16_t*)(ws + p.dz) : nullptr, rows_p, cols_p, part, vec);
         };
-        switch (activation) {
-            case NGPT_ACT_RELU2: go(std::integral_constant<int, NGPT_ACT_RELU2>{}); break;
-            case NGPT_ACT_GELU: go(std::integral_constant<int, NGPT_ACT_GELU>{}); break;
-            case NGPT_ACT_GELU_TANH: go(std::integral_constant<int, NGPT_ACT_GELU_TANH>{}); break;
-            case NGPT_ACT_SILU: go(std::integral_constant<int, NGPT_ACT_SILU>{}); break;
-            default: go(std::integral_constant<int, NGPT_ACT_NONE>{}); break;
-        }
+        with_act(activation, go);
         if (int e = check_launch("act_grad_kernel")) return e;
         if (dbias_bf16) {
             col_sum_kernel<<<(N + 31) / 32, kColSumThreads, 0, st>>>(part, p.sum_rows, N, (uint16_t*)dbias_bf16);
