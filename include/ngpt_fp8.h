@@ -341,13 +341,12 @@ int ngpt_lmhead_ce_bwd_codes(const void* x_f8, const void* w_f8_vk, const int64_
 /* ---- matrix product with bias, activation and residual in its epilogue ---------------------------
  * out [M, N] = residual + act(x [M, K] . w [N, K]^T + bias [N]), bf16 in and out, fp32 in between, rounded once.  bias and residual are nullable.
  * The bias starts on 16 bytes.
- * Row strides in elements; where K % 64 == 0 rows of x and w must start on 16 bytes (otherwise both are copied into the workspace).
+ * Row strides in elements, at most 2^21; rows may start anywhere (the fastest kernel for many rows needs K % 64 == 0 and rows of x and w on 16 bytes).
  * Any M, N, K.  pre [M, N] (nullable; null for NGPT_ACT_NONE) receives bf16(x w^T + bias), what the backward of an
  * activation needs. */
-int64_t ngpt_linear_act_fwd_workspace_bytes(int M, int N, int K);
 int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw, const void* bias_bf16,
                         const void* residual_bf16, int64_t ld_residual, int M, int N, int K, int activation,
-                        void* out_bf16, void* pre_bf16, void* workspace, int64_t workspace_bytes, void* stream);
+                        void* out_bf16, void* pre_bf16, void* stream);
 
 /* Its gradients from dout [M, N] (contiguous; it is the residual's gradient itself): dz = bf16(dout act'(pre)), dx [M, K] = dz w,
  * dw [N, K] = dz^T x, dbias [N] = sum of dout act'(pre) over the rows.  Each of the three outputs is nullable; pre may be null for

@@ -93,14 +93,6 @@ def _matrix(t: Tensor) -> Tensor:
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and _ld(t) >= t.shape[1] else t.contiguous()
 
 
-def _rows(t: Tensor) -> Tensor:
-    """The same with every row on 16 bytes where the row length allows it."""
-    t = _matrix(t)
-    if t.shape[1] % 64 == 0 and (_ld(t) % 8 or t.data_ptr() % 16):
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
-
-
 def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str, keep_pre: bool) -> tuple[Tensor, Tensor | None]:
     act = _linear_shapes(x, w, bias, residual, activation)
     assert act or not keep_pre, "keep_pre: without an activation the backward needs no pre-activation"
@@ -112,16 +104,12 @@ def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | No
         return out, pre
     if K == 0:
         raise RuntimeError("linear_act: contraction of length 0")
-    xr, wr = _rows(x), _rows(w)
+    xr, wr = _matrix(x), _matrix(w)
     if bias is not None and (bias.stride(0) != 1 or bias.data_ptr() % 16):
         bias = bias.clone(memory_format=torch.contiguous_format)
     res = None if residual is None else _matrix(residual)
-    lib = _lib.load()
-    M = xr.shape[0]
-    nws = lib.ngpt_linear_act_fwd_workspace_bytes(M, N, K)
-    ws = _workspace(nws, x.device) if nws else None
-    _launch(gpu, "ngpt_linear_act_fwd", _p(xr), _ld(xr), _p(wr), _ld(wr), _p(bias), _p(res), 0 if res is None else _ld(res), M, N, K, act,
-            _p(out), _p(pre), _p(ws), nws)
+    _launch(gpu, "ngpt_linear_act_fwd", _p(xr), _ld(xr), _p(wr), _ld(wr), _p(bias), _p(res), 0 if res is None else _ld(res), xr.shape[0], N, K, act,
+            _p(out), _p(pre))
     return out, pre
 
 
@@ -146,7 +134,7 @@ def _linear_bwd(dout: Tensor, x: Tensor, w: Tensor, pre: Tensor | None, activati
         return dx, dw, db
     dout = dout.contiguous()
     pre = None if pre is None else pre.contiguous()
-    xr, wr = _rows(x), _rows(w)
+    xr, wr = _matrix(x), _matrix(w)
     ws = _workspace(_lib.load().ngpt_linear_act_bwd_workspace_bytes(M, N, K), x.device)
     _launch(gpu, "ngpt_linear_act_bwd", _p(dout), _p(pre), _p(xr), _ld(xr), _p(wr), _ld(wr), M, N, K, act, _p(dx), _p(dw), _p(db), _p(ws), ws.numel())
     return dx, dw, db
@@ -219,7 +207,7 @@ class LinearActFunction(torch.autograd.Function):
 def linear_act(x: Tensor, w: Tensor, bias: Tensor | None = None, residual: Tensor | None = None, activation: str = "none") -> Tensor:
     """residual + act(x @ w.T + bias) for bf16 x [..., K], w [N, K], bias [N], residual [..., N]; fp32 accumulation, bias, activation
     and residual applied to the fp32 sums, one rounding.  `activation`: "none", "relu2" (max(z, 0)^2), "gelu", "gelu_tanh", "silu".
-    Any sizes (K % 64 == 0 reads the operands in place).  Differentiable in x, w, bias and residual; an activation's backward keeps
+    Any sizes; rows of x, w and residual may be strided.  Differentiable in x, w, bias and residual; an activation's backward keeps
     the bf16 pre-activation."""
     if not _plain(x, w, bias, residual):
         keep = activation != "none" and _needs_grad(x, w, bias)

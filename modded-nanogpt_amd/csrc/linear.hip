@@ -7,6 +7,7 @@
 #include "gemm_tn.h"
 #include "host_util.h"
 #include "launch.h"
+#include "linear.h"
 #include <algorithm>
 
 namespace ngpt {
@@ -17,103 +18,16 @@ int gemm_bf16_clipped(const void* A, int fa, int64_t lda, const void* B, int fb,
 
 namespace {
 
-// ---------------------------------------------------------------------------------------------- activations
-template <int ACT>
-__device__ __forceinline__ float act_of(float z) {
-    constexpr float kLog2e = 1.4426950408889634f;
-    if constexpr (ACT == NGPT_ACT_RELU2) {
-        const float r = fmaxf(z, 0.0f);
-        return z != z ? z : r * r;
-    } else if constexpr (ACT == NGPT_ACT_GELU) {
-        return z * (0.5f + 0.5f * erff(z * 0.70710678118654752f));
-    } else if constexpr (ACT == NGPT_ACT_GELU_TANH) {      // z (1 + tanh u) / 2 = z sigmoid(2 u)
-        const float u = z * __builtin_fmaf(z * z, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
-        return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.0f * kLog2e * u));
-    } else if constexpr (ACT == NGPT_ACT_SILU) {
-        return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
-    } else {
-        return z;
-    }
-}
-template <int ACT>
-__device__ __forceinline__ float act_slope(float z) {
-    constexpr float kLog2e = 1.4426950408889634f;
-    if constexpr (ACT == NGPT_ACT_RELU2) {
-        return z != z ? z : 2.0f * fmaxf(z, 0.0f);
-    } else if constexpr (ACT == NGPT_ACT_GELU) {
-        return 0.5f + 0.5f * erff(z * 0.70710678118654752f) + z * 0.3989422804014327f * __builtin_amdgcn_exp2f(-0.5f * kLog2e * z * z);
-    } else if constexpr (ACT == NGPT_ACT_GELU_TANH) {
-        const float u = z * __builtin_fmaf(z * z, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
-        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.0f * kLog2e * u));
-        return s + z * s * (1.0f - s) * 2.0f * __builtin_fmaf(z * z, 3.0f * 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
-    } else if constexpr (ACT == NGPT_ACT_SILU) {
-        const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
-        return s + z * s * (1.0f - s);
-    } else {
-        return 1.0f;
-    }
-}
-typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
-__device__ __forceinline__ float lo16(int w) { return __uint_as_float((uint32_t)w << 16); }
-__device__ __forceinline__ float hi16(int w) { return __uint_as_float((uint32_t)w & 0xffff0000u); }
-
-// 8 consecutive bf16 of a row, `n` of which exist; vec: one 16-byte access is allowed.  The value-by-value path is a loop on purpose: the
-// compiler stops inlining into a kernel of many basic blocks, and the GEMM's state then lives in scratch memory.
-__device__ __forceinline__ v4i load8(const uint16_t* p, int n, bool vec) {
-    if (vec && n >= 8) return *(const v4i*)p;
-    v4i w = {0, 0, 0, 0};
-#pragma unroll 1
-    for (int i = min(n, 8) - 1; i >= 0; --i) {
-        w.w = (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16);
-        w.z = (int)__builtin_amdgcn_alignbit((uint32_t)w.z, (uint32_t)w.y, 16);
-        w.y = (int)__builtin_amdgcn_alignbit((uint32_t)w.y, (uint32_t)w.x, 16);
-        w.x = (int)(((uint32_t)w.x << 16) | (uint32_t)p[i]);
-    }
-    return w;
-}
-__device__ __forceinline__ void store8(uint16_t* p, v4i w, int n, bool vec) {
-    if (vec && n >= 8) {
-        *(v4i*)p = w;
-        return;
-    }
-#pragma unroll 1
-    for (int i = 0; i < min(n, 8); ++i) {
-        p[i] = (uint16_t)w.x;
-        w.x = (int)__builtin_amdgcn_alignbit((uint32_t)w.y, (uint32_t)w.x, 16);
-        w.y = (int)__builtin_amdgcn_alignbit((uint32_t)w.z, (uint32_t)w.y, 16);
-        w.z = (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16);
-        w.w = (int)((uint32_t)w.w >> 16);
-    }
-}
-
 // ---------------------------------------------------------------------------------------------- epilogue of the tile GEMM
-// The product runs transposed (tile rows = output features, A = w; tile columns = rows of x, B = x): a lane then owns one row of
-// x and four consecutive features per accumulator register group.  Every 32-row x 64-feature block passes through the wave's 4 KiB
-// of LDS, so that z, the residual and the output cross memory as whole 128-byte lines.  16-byte pieces are XOR-swizzled by
-// the row; LDS operations of one wave execute in order, no waits are needed between the steps.
-// Memory is reached through descriptors of the tile's rows, whose bounds check stands for the branches at the matrix' end: a kernel of
-// many basic blocks is not inlined completely any more, and the GEMM's state then lives in scratch memory.  Rows that do not start on
-// 16 bytes are moved value by value, in loops.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_of(const void* base, int64_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, (int)(bytes < 0x7fffff00 ? bytes : 0x7fffff00), 0x00020000);
-}
-constexpr int kNowhere = 0x7ffffff0;      // an offset past any descriptor's end
-
 // One kernel an activation: five of them behind a switch in one kernel cost it 60 spilled registers.
-template <int WAVES, int ACT, bool PRE, bool RES>
+template <int ACT, bool PRE, bool RES>
 struct EpiLinear {
-    uint16_t* out;          // [C, R], row stride R
-    uint16_t* pre;          // PRE: z, same shape
-    const uint16_t* bias;   // nullable [R], on 16 bytes
-    const uint16_t* res;    // RES: [C, R], row stride ld_res
-    int64_t ld_res;
-    int R, C;
-    int vec, vec_res;       // rows of out and pre / of res start on 16 bytes and are whole 8-value pieces
-    static constexpr int EXTRA_LDS = WAVES * 4096;
+    LinearOut o;
+    static constexpr int EXTRA_LDS = 32768;         // 4 KiB per wave
     static constexpr bool NEEDS_SCRATCH = false;
     static constexpr bool JOB_END_NEEDS_SCRATCH = false;
     static constexpr bool DROPS_FRAGMENTS = true;   // the residual's lines in flight next to the accumulators
-    static constexpr int TILE_STORES = 8;           // at least: 4 per 32-row block and wave, 2 blocks or more (masked ones are issued too)
+    static constexpr int TILE_STORES = 16;          // at least: 4 per 32-row block and wave (those past the matrix' end are issued too)
     uint8_t* stage;
     bool stored_all;
     __device__ bool all_stores_issued() const { return stored_all; }
@@ -127,115 +41,11 @@ struct EpiLinear {
     __device__ void job_begin(int) {}
     template <class Cfg>
     __device__ void job_end(int, int, const AccCoords<Cfg>&, uint8_t*) {}
-
-    // the wave's block of 32 rows x 64 features, `row0` / `col0` its origin in the matrix, value by value
-    __device__ __forceinline__ void block_slow(const uint16_t* from, uint16_t* to, int64_t ld, int row0, int col0, int lane) {
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-            const int m = row0 + i, f = col0 + lane;
-            uint16_t* at = (uint16_t*)(stage + i * 128 + (((lane >> 3) ^ (i & 7)) << 4) + (lane & 7) * 2);
-            if (m < C && f < R) {
-                if (to) to[(int64_t)m * ld + f] = *at;
-                else *at = from[(int64_t)m * ld + f];
-            }
-        }
-    }
-
     template <class Cfg>
     __device__ __forceinline__ void tile(v16f (&acc)[Cfg::TM][Cfg::TN], int r0, int c0, const AccCoords<Cfg>& co, uint8_t*, int lane) {
-        static_assert(Cfg::TM == 2 && Cfg::TN >= 2 && Cfg::NWAVES == WAVES, "64-feature wave tiles, 4 KiB of staging each");
-        const int h = lane >> 5, j = lane & 31;
-        stored_all = vec != 0;
-        const int rd_row = lane >> 3, rd_chunk = lane & 7;
-        const int f = r0 + co.wave_row0 + rd_chunk * 8;          // this lane's 8 features in the line-wise steps
-        const int rows = C - c0;                                 // rows of the matrix from this tile on
-        const bool in = f < R;                                   // (R is a multiple of 8 where whole lines are moved)
-        const auto buf_out = buffer_of(out + (int64_t)c0 * R, (int64_t)rows * R * 2);
-        const auto buf_pre = buffer_of(PRE ? pre + (int64_t)c0 * R : out, PRE ? (int64_t)rows * R * 2 : 0);
-        const auto buf_res = buffer_of(RES ? res + (int64_t)c0 * ld_res : out, RES ? ((int64_t)(rows - 1) * ld_res + R) * 2 : 0);
-        const auto buf_bias = buffer_of(bias, bias ? ((int64_t)R * 2 + 3) & ~3ll : 0);
-        const int off = in ? ((co.wave_col0 + rd_row) * R + f) * 2 : kNowhere;
-        const int off_res = RES && in ? (int)(((co.wave_col0 + rd_row) * ld_res + f) * 2) : kNowhere;
-        v2i b[8];                                                // bias of the lane's features, packed
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-            b[i] = __builtin_bit_cast(v2i, __builtin_amdgcn_raw_buffer_load_b64(buf_bias, (r0 + co.wave_row0 + 8 * i + 4 * h) * 2, 0, 0));
-        v4i line[4];
-        auto load_block = [&](int tn) {
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-                line[k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(buf_res, in ? off_res + (int)((tn * 32 + 8 * k) * ld_res * 2) : kNowhere, 0, 0));
-        };
-        auto store_block = [&](int tn, __amdgpu_buffer_rsrc_t buf, uint16_t* to) {
-            if (vec) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const int row = 8 * k + rd_row;
-                    const v4i v = *(const v4i*)(stage + row * 128 + ((rd_chunk ^ (row & 7)) << 4));
-                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), buf, in ? off + (tn * 32 + 8 * k) * R * 2 : kNowhere, 0, 0);
-                }
-            } else {
-                block_slow(nullptr, to, R, c0 + co.wave_col0 + tn * 32, r0 + co.wave_row0, lane);
-            }
-        };
-        if constexpr (RES) { if (vec_res) load_block(0); }
-#pragma unroll
-        for (int tn = 0; tn < Cfg::TN; ++tn) {
-            const v16f* const a2[2] = {&acc[0][tn], &acc[1][tn]};
-            auto z_of = [&](int tm, int g, float (&z)[4]) {
-                const v16f& a = *a2[tm];
-                const v2i bb = b[tm * 4 + g];
-                z[0] = a[4 * g] + lo16(bb.x);
-                z[1] = a[4 * g + 1] + hi16(bb.x);
-                z[2] = a[4 * g + 2] + lo16(bb.y);
-                z[3] = a[4 * g + 3] + hi16(bb.y);
-            };
-            auto place = [&](int tm, int g) { return stage + j * 128 + (((tm * 4 + g) ^ (j & 7)) << 4) + 8 * h; };
-            if constexpr (PRE) {
-#pragma unroll
-                for (int tm = 0; tm < 2; ++tm)
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        float z[4];
-                        z_of(tm, g, z);
-                        *(v2i*)place(tm, g) = (v2i){(int)cvt_pk_bf16(z[0], z[1]), (int)cvt_pk_bf16(z[2], z[3])};
-                    }
-                store_block(tn, buf_pre, pre);
-            }
-            if constexpr (RES) {
-                if (vec_res) {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int row = 8 * k + rd_row;
-                        *(v4i*)(stage + row * 128 + ((rd_chunk ^ (row & 7)) << 4)) = line[k];
-                    }
-                    if (tn + 1 < Cfg::TN) load_block(tn + 1);       // in flight while this block is worked on
-                } else {
-                    block_slow(res, nullptr, ld_res, c0 + co.wave_col0 + tn * 32, r0 + co.wave_row0, lane);
-                }
-            }
-#pragma unroll
-            for (int tm = 0; tm < 2; ++tm)
-#pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    uint8_t* at = place(tm, g);
-                    float z[4];
-                    z_of(tm, g, z);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) z[i] = act_of<ACT>(z[i]);
-                    if constexpr (RES) {
-                        const v2i r = *(const v2i*)at;
-                        z[0] += lo16(r.x);
-                        z[1] += hi16(r.x);
-                        z[2] += lo16(r.y);
-                        z[3] += hi16(r.y);
-                    }
-                    *(v2i*)at = (v2i){(int)cvt_pk_bf16(z[0], z[1]), (int)cvt_pk_bf16(z[2], z[3])};
-                    if (g & 1) __builtin_amdgcn_sched_barrier(0);   // few temporaries next to the accumulators
-                }
-            store_block(tn, buf_out, out);
-            __builtin_amdgcn_sched_barrier(0);
-        }
+        static_assert(Cfg::TM == 2 && Cfg::TN == 4 && Cfg::NWAVES * 4096 <= EXTRA_LDS, "64 x 128 wave tiles, 4 KiB of staging each");
+        stored_all = o.vec != 0;
+        linear_epilogue<ACT, PRE, RES>(o, acc, stage, r0 + co.wave_row0, c0 + co.wave_col0, lane);
     }
 };
 
@@ -330,18 +140,6 @@ int act_grad_rows(int64_t M, int64_t N) {
     return (int)std::max<int64_t>(rows, 1);
 }
 
-// f(integral_constant) for the activation
-template <class F>
-auto with_act(int act, F&& f) {
-    switch (act) {
-        case NGPT_ACT_RELU2: return f(std::integral_constant<int, NGPT_ACT_RELU2>{});
-        case NGPT_ACT_GELU: return f(std::integral_constant<int, NGPT_ACT_GELU>{});
-        case NGPT_ACT_GELU_TANH: return f(std::integral_constant<int, NGPT_ACT_GELU_TANH>{});
-        case NGPT_ACT_SILU: return f(std::integral_constant<int, NGPT_ACT_SILU>{});
-        default: return f(std::integral_constant<int, NGPT_ACT_NONE>{});
-    }
-}
-
 int check_linear(const char* who, int M, int N, int K, int act) {
     if (M <= 0 || N <= 0 || K <= 0) return fail(NGPT_EINVAL, "%s: empty problem M=%d N=%d K=%d", who, M, N, K);
     if (act < NGPT_ACT_NONE || act > NGPT_ACT_SILU) return fail(NGPT_EINVAL, "%s: activation=%d", who, act);
@@ -349,22 +147,32 @@ int check_linear(const char* who, int M, int N, int K, int act) {
     return NGPT_OK;
 }
 
-// The tile GEMM reads rows that start on 16 bytes, a multiple of 64 values long: other operands are copied into the workspace first.
+// The 256 x 256 tile GEMM reads rows that start on 16 bytes, a multiple of 64 values long.
 bool rows_fit(const void* p, int64_t ld, int K) { return K % 64 == 0 && on16(p) && ld % 8 == 0; }
+
+int linear_big(const LinearOut& o, const void* x, int64_t ldx, const void* w, int64_t ldw, int K, int act, hipStream_t st) {
+    GemmOperands g{(const uint8_t*)w, (const uint8_t*)x, 2 * ldw, 2 * ldx, o.N, o.M, 2 * K, 1};
+    auto go = [&](auto epi) {
+        epi.o = o;
+        return launch_gemm_fmt<MainCfg, FMT_BF16, FMT_BF16>(g, epi, st, 0);
+    };
+    return with_act(act, [&](auto kind) {
+        constexpr int A = decltype(kind)::value;
+        if constexpr (A != NGPT_ACT_NONE) {
+            if (o.pre) return o.res ? go(EpiLinear<A, true, true>{}) : go(EpiLinear<A, true, false>{});
+        }
+        return o.res ? go(EpiLinear<A, false, true>{}) : go(EpiLinear<A, false, false>{});
+    });
+}
 
 }  // namespace
 }  // namespace ngpt
 
 using namespace ngpt;
 
-extern "C" int64_t ngpt_linear_act_fwd_workspace_bytes(int M, int N, int K) {
-    const int64_t Kp = up64(K);
-    return K % 64 ? align_up(((int64_t)M + N) * Kp * 2, 256) : 0;
-}
-
 extern "C" int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw, const void* bias_bf16,
                                    const void* residual_bf16, int64_t ld_residual, int M, int N, int K, int activation,
-                                   void* out_bf16, void* pre_bf16, void* workspace, int64_t workspace_bytes, void* stream) {
+                                   void* out_bf16, void* pre_bf16, void* stream) {
     const char* who = "ngpt_linear_act_fwd";
     if (!x_bf16 || !w_bf16 || !out_bf16) return fail(NGPT_EINVAL, "%s: null pointer", who);
     if (int e = check_linear(who, M, N, K, activation)) return e;
@@ -372,48 +180,20 @@ extern "C" int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* 
     if (!on16(bias_bf16)) return fail(NGPT_EALIGN, "%s: the bias starts on 16 bytes", who);
     if (ldx < K || ldw < K || (residual_bf16 && ld_residual < N))
         return fail(NGPT_EALIGN, "%s: row strides ldx=%lld ldw=%lld ld_residual=%lld", who, (long long)ldx, (long long)ldw, (long long)ld_residual);
+    // 32-bit offsets inside a tile
+    if (ldx > (1 << 21) || ldw > (1 << 21) || (residual_bf16 && ld_residual > (1 << 21)) || N > (1 << 21))
+        return fail(NGPT_ERANGE, "%s: row strides of at most 2^21 values (ldx=%lld ldw=%lld ld_residual=%lld N=%d)", who, (long long)ldx, (long long)ldw,
+                    (long long)ld_residual, N);
     hipStream_t st = (hipStream_t)stream;
-    const int64_t Kp = up64(K);
-    if (K % 64 == 0 && !(rows_fit(x_bf16, ldx, K) && rows_fit(w_bf16, ldw, K)))
-        return fail(NGPT_EALIGN, "%s: rows of x and w start on 16 bytes where K %% 64 == 0 (ldx=%lld ldw=%lld)", who, (long long)ldx, (long long)ldw);
-    if (K % 64) {
-        if (!workspace || workspace_bytes < ngpt_linear_act_fwd_workspace_bytes(M, N, K) || !on16(workspace))
-            return fail(NGPT_EWORKSPACE, "%s: workspace %lld < %lld bytes", who, (long long)workspace_bytes,
-                        (long long)ngpt_linear_act_fwd_workspace_bytes(M, N, K));
-        uint16_t* xp = (uint16_t*)workspace;
-        uint16_t* wp = xp + (int64_t)M * Kp;
-        if (int e = pad_copy(x_bf16, ldx, M, K, xp, M, Kp, st)) return e;
-        if (int e = pad_copy(w_bf16, ldw, N, K, wp, N, Kp, st)) return e;
-        x_bf16 = xp; w_bf16 = wp;
-        ldx = ldw = Kp;
-    }
+    LinearOut o{(uint16_t*)out_bf16, (uint16_t*)pre_bf16, (const uint16_t*)bias_bf16, (const uint16_t*)residual_bf16, ld_residual, M, N, 0, 0};
+    o.vec = N % 8 == 0 && on16(out_bf16) && on16(pre_bf16);
+    o.vec_res = residual_bf16 && N % 8 == 0 && ld_residual % 8 == 0 && on16(residual_bf16);
     ProfileScope prof(PROF_GEMM_BF16, st);
-    GemmOperands g{(const uint8_t*)w_bf16, (const uint8_t*)x_bf16, 2 * ldw, 2 * ldx, N, M, (int)(2 * Kp), 1};
-    auto go = [&](auto epi) {
-        using Epi = decltype(epi);
-        epi.out = (uint16_t*)out_bf16;
-        epi.pre = (uint16_t*)pre_bf16;
-        epi.bias = (const uint16_t*)bias_bf16;
-        epi.res = (const uint16_t*)residual_bf16;
-        epi.ld_res = ld_residual;
-        epi.R = N;
-        epi.C = M;
-        epi.vec = N % 8 == 0 && on16(out_bf16) && on16(pre_bf16);
-        epi.vec_res = residual_bf16 && N % 8 == 0 && ld_residual % 8 == 0 && on16(residual_bf16);
-        using Cfg = std::conditional_t<Epi::EXTRA_LDS == 8 * 4096, MainCfg, SmallCfg>;
-        return launch_gemm_fmt<Cfg, FMT_BF16, FMT_BF16>(g, epi, st, 0);
-    };
+    const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
+    if (M <= kFewRows) return linear_few(o, x, ldx, w, ldw, K, activation, st);
     const int64_t tiles = ((int64_t)(N + 255) / 256) * ((M + 255) / 256);
-    auto pick = [&](auto waves, auto kind) {
-        constexpr int W = decltype(waves)::value, A = decltype(kind)::value;
-        if constexpr (A != NGPT_ACT_NONE) {
-            if (pre_bf16) return residual_bf16 ? go(EpiLinear<W, A, true, true>{}) : go(EpiLinear<W, A, true, false>{});
-        }
-        return residual_bf16 ? go(EpiLinear<W, A, false, true>{}) : go(EpiLinear<W, A, false, false>{});
-    };
-    return with_act(activation, [&](auto kind) {
-        return 2 * tiles > num_cus() ? pick(std::integral_constant<int, 8>{}, kind) : pick(std::integral_constant<int, 4>{}, kind);
-    });
+    if (2 * tiles > num_cus() && rows_fit(x, ldx, K) && rows_fit(w, ldw, K)) return linear_big(o, x, ldx, w, ldw, K, activation, st);
+    return linear_mid(o, x, ldx, w, ldw, K, activation, st);
 }
 
 namespace ngpt {

@@ -23,16 +23,14 @@ def strides(*s):
 
 def test_linear_act_refusals(amd):
     lib = amd._lib.load()
-    fwd = lambda x=16, ldx=64, w=16, ldw=64, res=None, ldr=0, M=4, N=8, K=64, act=0, out=16, ws=None, nws=0: lib.ngpt_linear_act_fwd(
-        x, ldx, w, ldw, None, res, ldr, M, N, K, act, out, None, ws, nws, None)
+    fwd = lambda x=16, ldx=64, w=16, ldw=64, bias=None, res=None, ldr=0, M=4, N=8, K=64, act=0, out=16, pre=None: lib.ngpt_linear_act_fwd(
+        x, ldx, w, ldw, bias, res, ldr, M, N, K, act, out, pre, None)
     assert fwd(x=None) == -1 and fwd(w=None) == -1 and fwd(out=None) == -1
     assert fwd(M=0) == -1 and fwd(N=-1) == -1 and fwd(K=0) == -1
-    assert fwd(act=5) == -1 and fwd(act=-1) == -1
+    assert fwd(act=5) == -1 and fwd(act=-1) == -1 and fwd(pre=16) == -1
     assert fwd(ldx=63) == -2 and fwd(ldw=32) == -2 and fwd(res=16, ldr=7) == -2
-    assert fwd(ldx=68) == -2 and fwd(x=8) == -2 and b"16 bytes" in lib.ngpt_last_error()
-    assert fwd(N=1 << 25) == -4
-    assert fwd(K=65, ldx=65, ldw=65) == -3 and fwd(K=65, ldx=65, ldw=65, ws=16, nws=100) == -3
-    assert lib.ngpt_linear_act_fwd_workspace_bytes(4, 8, 64) == 0 and lib.ngpt_linear_act_fwd_workspace_bytes(4, 8, 65) >= 12 * 128 * 2
+    assert fwd(bias=8) == -2 and b"16 bytes" in lib.ngpt_last_error()
+    assert fwd(N=1 << 25) == -4 and fwd(ldx=1 << 22) == -4 and fwd(ldw=1 << 22) == -4 and fwd(res=16, ldr=1 << 22) == -4
     bwd = lambda dout=16, pre=None, x=16, w=16, M=4, N=8, K=64, act=0, dx=16, dw=16, db=16, ws=16, nws=1 << 40: lib.ngpt_linear_act_bwd(
         dout, pre, x, K, w, K, M, N, K, act, dx, dw, db, ws, nws, None)
     assert bwd(dout=None) == -1 and bwd(x=None) == -1 and bwd(w=None) == -1 and bwd(act=2) == -1 and bwd(M=0) == -1
