@@ -94,7 +94,7 @@ auto with_act(int act, F&& f) {
 // the row; LDS operations of one wave execute in order, no waits are needed between the steps.
 // Memory is reached through descriptors of the wave's rows, whose bounds check stands for the branches at the matrix' end: a kernel of
 // many basic blocks is not inlined completely any more, and a GEMM's state then lives in scratch memory.  Rows that do not start on
-// 16 bytes are moved value by value, in loops.
+// 16 bytes go without descriptors, in a loop.
 struct LinearOut {
     uint16_t* out;          // [M, N], row stride N
     uint16_t* pre;          // nullable; z, same shape
@@ -137,15 +137,24 @@ __device__ __forceinline__ void linear_epilogue(const LinearOut& o, v16f (&acc)[
             line[k] = __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(
                 buf_res, in ? off_res + (tn * 32 + RPI * k) * (int)o.ld_res * 2 : kNowhere, 0, 0));
     };
-    // a block value by value, between memory and the staging area
+    // a block between memory and the staging area where rows start anywhere: 16 bytes at any byte address, the row's last values one by one
     auto block_slow = [&](int tn, const uint16_t* from, uint16_t* to, int64_t ld) {
 #pragma unroll 1
-        for (int i = 0; i < 16 * TM; ++i) {
-            const int row = (i * 64 + lane) / (32 * TM), c = (i * 64 + lane) % (32 * TM), m = m0 + tn * 32 + row;
-            uint16_t* at = (uint16_t*)(stage + swz(row, c >> 3) + (c & 7) * 2);
-            if (m < o.M && f0 + c < N) {
-                if (to) to[(int64_t)m * ld + f0 + c] = *at;
-                else *at = from[(int64_t)m * ld + f0 + c];
+        for (int k = 0; k < NI; ++k) {
+            const int row = RPI * k + rd_row, m = m0 + tn * 32 + row, left = N - f;
+            uint8_t* at = stage + swz(row, rd_chunk);
+            if (m < o.M && left > 0) {
+                const int64_t i = (int64_t)m * ld + f;
+                if (to) {
+                    const v4i v = *(const v4i*)at;
+                    if (left >= 8) __builtin_memcpy(to + i, &v, 16);
+                    else store8(to + i, v, left, false);
+                } else {
+                    v4i v;
+                    if (left >= 8) __builtin_memcpy(&v, from + i, 16);
+                    else v = load8(from + i, left, false);
+                    *(v4i*)at = v;
+                }
             }
         }
     };
@@ -218,7 +227,7 @@ __device__ __forceinline__ void linear_epilogue(const LinearOut& o, v16f (&acc)[
 }
 
 // linear_small.hip: any alignment, any K.  The few-row kernel takes M <= kFewRows.
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 32;
 int linear_few(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int K, int act, hipStream_t st);
 int linear_mid(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int K, int act, hipStream_t st);
 

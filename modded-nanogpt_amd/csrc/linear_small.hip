@@ -3,6 +3,7 @@
 // Loads go through registers here, 16 bytes at any byte address (gfx950 takes unaligned global loads), so rows may start anywhere and K is any
 // length; only a row's last, incomplete piece is read value by value.
 #include "linear.h"
+#include "launch.h"
 #include <algorithm>
 
 namespace ngpt {
@@ -28,7 +29,7 @@ __device__ __forceinline__ void act_switch(int act, F&& f) {      // wave-unifor
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
-// Every weight is read once and used for at most 64 rows: the bound is the weights' way from memory, and for one token the launch and one
+// Every weight is read once and used for at most 32 rows: the bound is the weights' way from memory, and for one token the launch and one
 // round trip.  A workgroup owns 16 FT features; its waves share the contraction in units of 64 values (a line of every weight row), with all
 // loads of U units in flight, multiply on 16x16x32 matrix instructions (rows past M repeat the last and are dropped) and add up through LDS
 // in wave order.
@@ -117,24 +118,28 @@ __global__ __launch_bounds__(1024) void linear_few_kernel(LinearOut o, const uin
 }
 
 // ---------------------------------------------------------------------------------------------- tiles of 128 x 128 or 64 x 64
-// Four waves as 2 x 2, TM x TM matrix tiles of 32 x 32 each.  A k-step is 64 values: rows of 128 bytes in LDS, their eight 16-byte pieces
-// swizzled by the row as in gemm_tn.h.  Operands pass through registers, loaded two k-steps ahead of their use; two LDS stages, one barrier a
-// k-step.  Several workgroups share a compute unit and cover each other's latencies.
-template <int TM>
+// KG groups of four waves share a tile and cut its contraction between them; each group works as 2 x 2 waves of TM x TM matrix tiles of 32 x 32
+// with LDS stages of its own, and the groups' sums meet in LDS, in order.  A k-step is 64 values: rows of 128 bytes in LDS, their eight 16-byte
+// pieces swizzled by the row as in gemm_tn.h.  Operands pass through registers, requested three k-steps ahead of their use; two LDS stages, one
+// barrier a k-step.  A k-step of one group is mostly latency: several groups or workgroups on a compute unit cover each other's.
+template <int TM, int KG>
 struct MidCfg {
     static constexpr int B = 64 * TM;                 // tile edge
     static constexpr int LOADS = 2 * B * 8 / 256;     // 16-byte pieces a thread moves per k-step, A then B
     static constexpr int STAGE = 2 * B * 128;         // bytes
-    static constexpr int SMEM = 2 * STAGE;
+    static constexpr int SMEM = 2 * STAGE * KG;
+    static constexpr int THREADS = 256 * KG;
 };
 
-template <int TM, bool PRE, bool RES>
-__global__ __launch_bounds__(256, 2) void linear_mid_kernel(LinearOut o, const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ w,
-                                                            int64_t ldw, int K, int act) {
-    using Cfg = MidCfg<TM>;
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[Cfg::SMEM];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+template <int TM, int KG, bool PRE, bool RES>
+__global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : 2) void linear_mid_kernel(LinearOut o, const uint16_t* __restrict__ x, int64_t ldx,
+                                                                               const uint16_t* __restrict__ w, int64_t ldw, int K, int act) {
+    using Cfg = MidCfg<TM, KG>;
+    extern __shared__ __attribute__((aligned(1024))) uint8_t smem_all[];
+    const int tid = threadIdx.x & 255, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int kg = __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
     const int wr = wave >> 1, wc = wave & 1;
+    uint8_t* const smem = smem_all + kg * 2 * Cfg::STAGE;
     // tiles in runs of consecutive numbers per XCD (workgroup b runs on XCD b % 8); features fastest inside groups of 8 row tiles
     const int tf = (o.N + Cfg::B - 1) / Cfg::B, tm = (o.M + Cfg::B - 1) / Cfg::B, total = tf * tm;
     int t = blockIdx.x;
@@ -153,11 +158,11 @@ __global__ __launch_bounds__(256, 2) void linear_mid_kernel(LinearOut o, const u
     }
     const uint16_t* const wt = w + (int64_t)f0 * ldw;
     const uint16_t* const xt = x + (int64_t)m0 * ldx;
-    v4i reg[Cfg::LOADS];
-    const int steps = (K + 63) / 64;
-    auto load = [&](int kt) {
-        const int k = kt * 64 + chunk * 8;
-        if (kt * 64 + 64 <= K) {
+    const int steps = (K + 63) / 64, mine = (steps + KG - 1) / KG, kt0 = kg * mine;      // every group walks `mine` steps, empty ones included
+    auto load = [&](int kt, v4i (&reg)[Cfg::LOADS]) {
+        const int k = (kt0 + kt) * 64 + chunk * 8;
+        if (kt >= mine) return;
+        if ((kt0 + kt) * 64 + 64 <= K) {
 #pragma unroll
             for (int i = 0; i < Cfg::LOADS; ++i) __builtin_memcpy(&reg[i], (i < Cfg::LOADS / 2 ? wt : xt) + off[i] + k, 16);
         } else {
@@ -165,7 +170,7 @@ __global__ __launch_bounds__(256, 2) void linear_mid_kernel(LinearOut o, const u
             for (int i = 0; i < Cfg::LOADS; ++i) reg[i] = load_k8((i < Cfg::LOADS / 2 ? wt : xt) + off[i], k, K);
         }
     };
-    auto put = [&](int stage) {
+    auto put = [&](int stage, const v4i (&reg)[Cfg::LOADS]) {
         uint8_t* s = smem + stage * Cfg::STAGE;
 #pragma unroll
         for (int i = 0; i < Cfg::LOADS; ++i) {
@@ -185,13 +190,12 @@ __global__ __launch_bounds__(256, 2) void linear_mid_kernel(LinearOut o, const u
         fa[i] = ra * 128 + (((lane >> 5) ^ ((ra >> 1) & 7)) << 4);
         fb[i] = rb * 128 + (((lane >> 5) ^ ((rb >> 1) & 7)) << 4);
     }
-    load(0);
-    put(0);
-    if (steps > 1) load(1);
-    for (int kt = 0; kt < steps; ++kt) {
+    v4i even[Cfg::LOADS], odd[Cfg::LOADS];
+    // one k-step: `reg` holds step kt + 1 and is refilled with step kt + 3
+    auto step = [&](int kt, v4i (&reg)[Cfg::LOADS]) {
         wg_barrier();                                // stage kt % 2 is complete, stage (kt + 1) % 2 has been read
-        if (kt + 1 < steps) put((kt + 1) & 1);
-        if (kt + 2 < steps) load(kt + 2);
+        if (kt + 1 < mine) put((kt + 1) & 1, reg);
+        load(kt + 3, reg);
         const uint8_t* s = smem + (kt & 1) * Cfg::STAGE;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {             // 16 values: chunks 2 ks, 2 ks + 1
@@ -205,9 +209,48 @@ __global__ __launch_bounds__(256, 2) void linear_mid_kernel(LinearOut o, const u
 #pragma unroll
                 for (int j = 0; j < TM; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a[i], b[j], acc[i][j], 0, 0, 0);
         }
+    };
+    load(0, even);
+    put(0, even);
+    load(1, odd);
+    load(2, even);
+    for (int kt = 0; kt < mine; kt += 2) {
+        step(kt, odd);
+        if (kt + 1 < mine) step(kt + 1, even);
     }
-    wg_barrier();                                    // the stages become the waves' staging areas
-    uint8_t* const stage = smem + wave * 2048 * TM;
+    wg_barrier();                                    // the stages are free
+    if constexpr (KG > 1) {
+        // groups 1 .. leave their sums: [group][wave][tile][quarter][lane] of 16 bytes
+        v4f* const part = (v4f*)smem_all;
+        if (kg > 0) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TM; ++j)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v)
+                        part[((((kg - 1) * 4 + wave) * TM * TM + i * TM + j) * 4 + v) * 64 + lane] =
+                            (v4f){acc[i][j][4 * v], acc[i][j][4 * v + 1], acc[i][j][4 * v + 2], acc[i][j][4 * v + 3]};
+        }
+        wg_barrier();
+        if (kg > 0) return;
+#pragma unroll
+        for (int g = 0; g < KG - 1; ++g)
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TM; ++j)
+#pragma unroll
+                    for (int v = 0; v < 4; ++v) {
+                        const v4f p = part[(((g * 4 + wave) * TM * TM + i * TM + j) * 4 + v) * 64 + lane];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc[i][j][4 * v + e] += p[e];
+                    }
+    }
+    // staging areas of the remaining waves, behind the sums
+    constexpr int kSums = (KG - 1) * 4 * TM * TM * 4096;
+    static_assert(kSums + 4 * 2048 * TM <= Cfg::SMEM, "sums and staging areas fit the stages");
+    uint8_t* const stage = smem_all + kSums + wave * 2048 * TM;
     act_switch(act, [&](auto kind) {
         linear_epilogue<decltype(kind)::value, PRE, RES>(o, acc, stage, f0 + wr * 32 * TM, m0 + wc * 32 * TM, lane);
     });
@@ -233,22 +276,40 @@ int linear_few(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_
     std::integral_constant<int, 2> c2;
     std::integral_constant<int, 4> c4;
     if (o.M <= 16) return go(c1, c1, c4);
-    if (o.M <= 32) return go(c1, c2, c2);
-    return go(c1, c4, c2);
+    return go(c1, c2, c2);
 }
 
 int linear_mid(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int K, int act, hipStream_t st) {
-    auto go = [&](auto tm_c) {
-        constexpr int TM = decltype(tm_c)::value, B = MidCfg<TM>::B;
-        const int64_t tiles = (int64_t)((o.N + B - 1) / B) * ((o.M + B - 1) / B);
+    const int cus = num_cus();
+    if (cus <= 0) return fail(NGPT_EINVAL, "no HIP device");
+    auto go = [&](auto tm_c, auto kg_c) {
+        constexpr int TM = decltype(tm_c)::value, KG = decltype(kg_c)::value;
+        using Cfg = MidCfg<TM, KG>;
+        const int64_t tiles = (int64_t)((o.N + Cfg::B - 1) / Cfg::B) * ((o.M + Cfg::B - 1) / Cfg::B);
         if (tiles > 0x7fffffff) return fail(NGPT_ERANGE, "linear_mid: M=%d N=%d", o.M, o.N);
-        auto run = [&](auto kernel) { kernel<<<(unsigned)tiles, 256, 0, st>>>(o, x, ldx, w, ldw, K, act); };
-        if (o.pre) o.res ? run(linear_mid_kernel<TM, true, true>) : run(linear_mid_kernel<TM, true, false>);
-        else o.res ? run(linear_mid_kernel<TM, false, true>) : run(linear_mid_kernel<TM, false, false>);
-        return check_launch("linear_mid_kernel");
+        auto run = [&](auto pre, auto res) {
+            auto kernel = linear_mid_kernel<TM, KG, decltype(pre)::value, decltype(res)::value>;
+            static PerDeviceOnce configured;         // one per instantiation of this lambda, i.e. per kernel
+            if (int e = configured.run([&] { return allow_lds(kernel, Cfg::SMEM); })) return e;
+            kernel<<<(unsigned)tiles, Cfg::THREADS, Cfg::SMEM, st>>>(o, x, ldx, w, ldw, K, act);
+            return check_launch("linear_mid_kernel");
+        };
+        std::true_type yes;
+        std::false_type no;
+        if (o.pre) return o.res ? run(yes, yes) : run(yes, no);
+        return o.res ? run(no, yes) : run(no, no);
     };
-    const int64_t big = (int64_t)((o.N + 127) / 128) * ((o.M + 127) / 128);
-    return big >= 4 * (int64_t)num_cus() ? go(std::integral_constant<int, 2>{}) : go(std::integral_constant<int, 1>{});
+    std::integral_constant<int, 1> c1;
+    std::integral_constant<int, 2> c2;
+    std::integral_constant<int, 4> c4;
+    auto tiles = [&](int b) { return (int64_t)((o.N + b - 1) / b) * ((o.M + b - 1) / b); };
+    if (tiles(128) >= 2 * (int64_t)cus) return go(c2, c1);
+    // tiles of 64: about sixteen waves a compute unit
+    const int64_t t64 = tiles(64);
+    const int steps = (K + 63) / 64;
+    if (t64 >= 3 * (int64_t)cus || steps < 4) return go(c1, c1);
+    if (t64 > cus || steps < 8) return go(c1, c2);
+    return go(c1, c4);
 }
 
 }  // namespace ngpt
