@@ -52,14 +52,40 @@ struct EpiLinear {
 // ---------------------------------------------------------------------------------------------- around the products
 // dst [rows_p, cols_p] = src [rows, cols] with zeros around it; cols_p % 8 == 0.
 __global__ __launch_bounds__(256) void pad_copy_kernel(const uint16_t* __restrict__ src, int64_t ld, int rows, int cols, uint16_t* __restrict__ dst,
-                                                       int rows_p, int cols_p, int vec) {
+                                                       int rows_p, int cols_p) {
     const int c8 = cols_p / 8;
     const int64_t n = (int64_t)rows_p * c8;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int r = (int)(i / c8), c = (int)(i - (int64_t)r * c8) * 8;
         v4i w = {0, 0, 0, 0};
-        if (r < rows) w = load8(src + (int64_t)r * ld + c, cols - c, vec != 0);
+        if (r < rows && c < cols) w = load_any(src + (int64_t)r * ld + c, cols - c);
         *(v4i*)(dst + i * 8) = w;
+    }
+}
+
+// dst [cols, rows_p] = transpose of src [rows, cols], zeros behind its rows; rows_p % 64 == 0.  64 x 64 blocks through LDS: 16-byte pieces in
+// (at any address) and out.
+__global__ __launch_bounds__(256) void transpose_pad_kernel(const uint16_t* __restrict__ src, int64_t ld, int rows, int cols, uint16_t* __restrict__ dst,
+                                                            int rows_p) {
+    __shared__ uint16_t tile[64][64 + 4];
+    const int r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, t = threadIdx.x;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int r = (t >> 3) + 32 * i, c = (t & 7) * 8, left = cols - c0 - c;
+        v4i w = {0, 0, 0, 0};
+        if (r0 + r < rows && left > 0) w = load_any(src + (int64_t)(r0 + r) * ld + c0 + c, left);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) *(uint32_t*)&tile[r][c + 2 * e] = (uint32_t)w[e];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const int c = (t >> 3) + 32 * i, r = (t & 7) * 8;
+        if (c0 + c >= cols) continue;
+        v4i w;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = (int)((uint32_t)tile[r + 2 * e][c] | ((uint32_t)tile[r + 2 * e + 1][c] << 16));
+        *(v4i*)(dst + (int64_t)(c0 + c) * rows_p + r0 + r) = w;
     }
 }
 
@@ -68,7 +94,7 @@ __global__ __launch_bounds__(256) void pad_copy_kernel(const uint16_t* __restric
 constexpr int kColsPerBlock = 256, kRowLanes = 8;
 template <int ACT>
 __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restrict__ dout, const uint16_t* __restrict__ pre, int M, int N,
-                                                       uint16_t* __restrict__ dz, int rows_p, int cols_p, float* __restrict__ part, int vec) {
+                                                       uint16_t* __restrict__ dz, int rows_p, int cols_p, float* __restrict__ part) {
     __shared__ float red[kRowLanes][kColsPerBlock + 4];
     const int ct = threadIdx.x & 31, rt = threadIdx.x >> 5;
     const int c = blockIdx.x * kColsPerBlock + ct * 8;
@@ -77,7 +103,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restric
         for (int r = blockIdx.y * kRowLanes + rt; r < rows_p; r += gridDim.y * kRowLanes) {
             v4i g = {0, 0, 0, 0}, o = {0, 0, 0, 0};
             if (r < M && c < N) {
-                g = load8(dout + (int64_t)r * N + c, N - c, vec != 0);
+                g = load_any(dout + (int64_t)r * N + c, N - c);
                 if constexpr (ACT == NGPT_ACT_NONE) {
                     o = g;
 #pragma unroll
@@ -86,7 +112,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restric
                         sum[2 * i + 1] += hi16(g[i]);
                     }
                 } else {
-                    const v4i z = load8(pre + (int64_t)r * N + c, N - c, vec != 0);
+                    const v4i z = load_any(pre + (int64_t)r * N + c, N - c);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float d0 = lo16(g[i]) * act_slope<ACT>(lo16(z[i])), d1 = hi16(g[i]) * act_slope<ACT>(hi16(z[i]));
@@ -128,9 +154,14 @@ int pad_copy(const void* src, int64_t ld, int64_t rows, int64_t cols, void* dst,
     const int64_t n = rows_p * cols_p / 8;
     const int64_t cap = (int64_t)std::max(num_cus(), 1) * 16;
     const int grid = (int)std::min<int64_t>((n + 255) / 256, cap);
-    pad_copy_kernel<<<grid, 256, 0, st>>>((const uint16_t*)src, ld, (int)rows, (int)cols, (uint16_t*)dst, (int)rows_p, (int)cols_p,
-                                          on16(src) && ld % 8 == 0);
+    pad_copy_kernel<<<grid, 256, 0, st>>>((const uint16_t*)src, ld, (int)rows, (int)cols, (uint16_t*)dst, (int)rows_p, (int)cols_p);
     return check_launch("pad_copy_kernel");
+}
+
+int transpose_pad(const uint16_t* src, int64_t ld, int rows, int cols, uint16_t* dst, int rows_p, hipStream_t st) {
+    if ((cols + 63) / 64 > 65535) return fail(NGPT_ERANGE, "transpose_pad: %d columns", cols);
+    transpose_pad_kernel<<<dim3(rows_p / 64, (cols + 63) / 64), 256, 0, st>>>(src, ld, rows, cols, dst, rows_p);
+    return check_launch("transpose_pad_kernel");
 }
 
 // Workgroups along the rows of act_grad_kernel, whatever the device
@@ -165,6 +196,14 @@ int linear_big(const LinearOut& o, const void* x, int64_t ldx, const void* w, in
     });
 }
 
+// Which kernel: few rows; enough 256 x 256 tiles for half the compute units, in a form that kernel reads; anything else.
+int linear_run(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int K, int act, hipStream_t st) {
+    if (o.M <= kFewRows) return linear_few(o, x, ldx, w, ldw, K, act, st);
+    const int64_t tiles = ((int64_t)(o.N + 255) / 256) * ((o.M + 255) / 256);
+    if (2 * tiles > num_cus() && rows_fit(x, ldx, K) && rows_fit(w, ldw, K)) return linear_big(o, x, ldx, w, ldw, K, act, st);
+    return linear_mid(o, x, ldx, w, ldw, K, act, st);
+}
+
 }  // namespace
 }  // namespace ngpt
 
@@ -189,16 +228,12 @@ extern "C" int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* 
     o.vec = N % 8 == 0 && on16(out_bf16) && on16(pre_bf16);
     o.vec_res = residual_bf16 && N % 8 == 0 && ld_residual % 8 == 0 && on16(residual_bf16);
     ProfileScope prof(PROF_GEMM_BF16, st);
-    const uint16_t *x = (const uint16_t*)x_bf16, *w = (const uint16_t*)w_bf16;
-    if (M <= kFewRows) return linear_few(o, x, ldx, w, ldw, K, activation, st);
-    const int64_t tiles = ((int64_t)(N + 255) / 256) * ((M + 255) / 256);
-    if (2 * tiles > num_cus() && rows_fit(x, ldx, K) && rows_fit(w, ldw, K)) return linear_big(o, x, ldx, w, ldw, K, activation, st);
-    return linear_mid(o, x, ldx, w, ldw, K, activation, st);
+    return linear_run(o, (const uint16_t*)x_bf16, ldx, (const uint16_t*)w_bf16, ldw, K, activation, st);
 }
 
 namespace ngpt {
 namespace {
-// Workspace of the backward: dz [M64, N64] | w [N64, K8] | x [M64, K8] (copies of what the products cannot read in place) | parts of split
+// Workspace of the backward: dz [M64, N64] | w^T [K, N64] | x [M64, K8] (a copy where dw's product cannot read x in place) | parts of dw's split
 // tiles | column sums
 struct BwdPlan {
     int64_t M64, N64, K8, dz, w, x, parts, sums, total;
@@ -207,9 +242,9 @@ struct BwdPlan {
         M64 = up64(M); N64 = up64(N); K8 = up8(K);
         dz = 0;
         w = dz + align_up(M64 * N64 * 2, 256);
-        x = w + align_up(N64 * K8 * 2, 256);
+        x = w + align_up(N64 * K * 2, 256);
         parts = x + align_up(M64 * K8 * 2, 256);
-        sums = parts + align_up(std::max(balanced_part_bytes(M, (int)K8, (int)(2 * N64)), balanced_part_bytes((int)N64, (int)K8, (int)(2 * M64))), 256);
+        sums = parts + align_up(balanced_part_bytes((int)N64, (int)K8, (int)(2 * M64)), 256);
         sum_rows = act_grad_rows(M, N);
         total = sums + align_up((int64_t)sum_rows * N * 4, 256);
     }
@@ -235,18 +270,17 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
         return fail(NGPT_EWORKSPACE, "%s: workspace %lld < %lld bytes", who, (long long)workspace_bytes, (long long)p.total);
     hipStream_t st = (hipStream_t)stream;
     uint8_t* ws = (uint8_t*)workspace;
-    const bool need_gemm = dx_bf16 || dw_bf16;
     // dz is dout itself where there is no activation and the products can read it in place
-    const bool own_dz = need_gemm && !(activation == NGPT_ACT_NONE && M % 64 == 0 && N % 64 == 0 && on16(dout_bf16));
+    const bool own_dz = (dx_bf16 || dw_bf16) && (activation != NGPT_ACT_NONE || !on16(dout_bf16) || (dw_bf16 && (M % 64 || N % 8)));
     const uint16_t* dz = own_dz ? (const uint16_t*)(ws + p.dz) : (const uint16_t*)dout_bf16;
+    const int64_t ld_dz = own_dz ? p.N64 : N;
     if (own_dz || dbias_bf16) {
-        const int vec = N % 8 == 0 && on16(dout_bf16) && on16(pre_bf16);
         const int rows_p = own_dz ? (int)p.M64 : M, cols_p = own_dz ? (int)p.N64 : (int)up8(N);
         float* part = dbias_bf16 ? (float*)(ws + p.sums) : nullptr;
         const dim3 grid((cols_p + kColsPerBlock - 1) / kColsPerBlock, p.sum_rows);
         auto go = [&](auto kind) {
             act_grad_kernel<decltype(kind)::value><<<grid, 256, 0, st>>>((const uint16_t*)dout_bf16, (const uint16_t*)pre_bf16, M, N,
-                                                                         own_dz ? (uint16_t*)(ws + p.dz) : nullptr, rows_p, cols_p, part, vec);
+                                                                         own_dz ? (uint16_t*)(ws + p.dz) : nullptr, rows_p, cols_p, part);
         };
         with_act(activation, go);
         if (int e = check_launch("act_grad_kernel")) return e;
@@ -256,16 +290,13 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
         }
     }
     GemmSlot slot(PROF_GEMM_BF16);
-    float* parts = (float*)(ws + p.parts);
-    if (dx_bf16) {      // dx [M, K] = dz . w, contraction over the N rows of w
-        const void* w = w_bf16;
-        if (N % 64 || K % 8 || ldw % 8 || !on16(w)) {
-            if (int e = pad_copy(w_bf16, ldw, N, K, ws + p.w, p.N64, p.K8, st)) return e;
-            w = ws + p.w;
-            ldw = p.K8;
-        }
-        if (int e = gemm_bf16_clipped(dz, FMT_BF16, 2 * p.N64, w, FMT_BF16 | FMT_TRANSPOSED, 2 * ldw, M, (int)p.K8, (int)(2 * p.N64), M, K, dx_bf16, K,
-                                      parts, st)) return e;
+    if (dx_bf16) {
+        // dx [M, K] = dz . w: as a forward product with w^T, one pass over w more, but both operands then have the contraction contiguous
+        uint16_t* wt = (uint16_t*)(ws + p.w);
+        if (int e = transpose_pad((const uint16_t*)w_bf16, ldw, N, K, wt, (int)p.N64, st)) return e;
+        LinearOut o{(uint16_t*)dx_bf16, nullptr, nullptr, nullptr, 0, M, K, K % 8 == 0 && on16(dx_bf16), 0};
+        // (dz's padding and w^T's are zeros)
+        if (int e = linear_run(o, dz, ld_dz, wt, p.N64, own_dz ? (int)p.N64 : N, NGPT_ACT_NONE, st)) return e;
     }
     if (dw_bf16) {      // dw [N, K] = dz^T . x, contraction over the M rows of both
         const void* x = x_bf16;
@@ -274,8 +305,8 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
             x = ws + p.x;
             ldx = p.K8;
         }
-        if (int e = gemm_bf16_clipped(dz, FMT_BF16 | FMT_TRANSPOSED, 2 * p.N64, x, FMT_BF16 | FMT_TRANSPOSED, 2 * ldx, (int)p.N64, (int)p.K8,
-                                      (int)(2 * p.M64), N, K, dw_bf16, K, parts, st)) return e;
+        if (int e = gemm_bf16_clipped(dz, FMT_BF16 | FMT_TRANSPOSED, 2 * ld_dz, x, FMT_BF16 | FMT_TRANSPOSED, 2 * ldx, (int)(own_dz ? p.N64 : N), (int)p.K8,
+                                      (int)(2 * p.M64), N, K, dw_bf16, K, (float*)(ws + p.parts), st)) return e;
     }
     return NGPT_OK;
 }

@@ -10,12 +10,7 @@ namespace ngpt {
 namespace {
 
 // values k .. k + 7 of a row of K; zeros behind its end
-__device__ __forceinline__ v4i load_k8(const uint16_t* row, int k, int K) {
-    v4i w = {0, 0, 0, 0};
-    if (k + 8 <= K) __builtin_memcpy(&w, row + k, 16);
-    else if (k < K) w = load8(row + k, K - k, false);
-    return w;
-}
+__device__ __forceinline__ v4i load_k8(const uint16_t* row, int k, int K) { return k < K ? load_any(row + k, K - k) : (v4i){0, 0, 0, 0}; }
 
 template <class F>
 __device__ __forceinline__ void act_switch(int act, F&& f) {      // wave-uniform
