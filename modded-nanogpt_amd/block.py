@@ -24,6 +24,7 @@ from .ops import _p, _workspace
 # the current stream's handle without the Stream object around it
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)       # (a tensor on a GPU is there: CUDA is initialised)
 
 ACTIVATIONS = {"none": 0, "relu2": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 RMS_EPS = 1.1920928955078125e-07          # machine epsilon of fp32, what the other norms of this package add
@@ -33,18 +34,25 @@ _DTYPES = {torch.bfloat16: _lib.DT_BF16, torch.float32: _lib.DT_F32}
 def _same_gpu(first: Tensor, *others: Tensor | None) -> int:
     """Index of the GPU that holds all of them."""
     index = first.get_device()
-    for t in (first, *others):
-        if t is not None and t.get_device() != index or index < 0:
-            if t is None or t.is_cuda and index >= 0:
-                raise AssertionError(f"tensors on {first.device} and {t.device}")
-            raise RuntimeError("nanogpt operators run on the GPU only (got a CPU tensor); there is no CPU fallback")
+    if index < 0:
+        raise RuntimeError("nanogpt operators run on the GPU only (got a CPU tensor); there is no CPU fallback")
+    for t in others:
+        if t is not None and t.get_device() != index:
+            if not t.is_cuda:
+                raise RuntimeError("nanogpt operators run on the GPU only (got a CPU tensor); there is no CPU fallback")
+            raise AssertionError(f"tensors on {first.device} and {t.device}")
     return index
+
+
+_entry_points: dict = {}
 
 
 def _launch(index: int, what: str, *args) -> None:
     """Calls an entry point on GPU `index` and its current stream."""
-    fn = getattr(_lib.load(), what)
-    if index == torch.cuda.current_device():
+    fn = _entry_points.get(what)
+    if fn is None:
+        fn = _entry_points[what] = getattr(_lib.load(), what)
+    if index == _current_device():
         code = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
@@ -73,13 +81,19 @@ def _needs_grad(*tensors: Tensor | None) -> bool:
 # linear_act
 
 def _linear_shapes(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | None, activation: str) -> int:
-    assert activation in ACTIVATIONS, f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}"
-    assert w.ndim == 2 and x.ndim >= 1 and x.shape[-1] == w.shape[1], f"x {tuple(x.shape)} and w {tuple(w.shape)}: x is [..., K], w [N, K]"
-    assert bias is None or bias.shape == (w.shape[0],), f"bias {tuple(bias.shape)}: one value per row of w"
-    assert residual is None or residual.shape == (*x.shape[:-1], w.shape[0]), f"residual {tuple(residual.shape)}: the shape of the result"
-    for t in (x, w, bias, residual):
-        assert t is None or t.dtype == torch.bfloat16, f"linear_act takes bfloat16, got {t.dtype}"
-    return ACTIVATIONS[activation]
+    act = ACTIVATIONS.get(activation)
+    assert act is not None, f"activation {activation!r}: one of {', '.join(ACTIVATIONS)}"
+    xs, ws = x.shape, w.shape
+    assert len(ws) == 2 and len(xs) >= 1 and xs[-1] == ws[1], f"x {tuple(xs)} and w {tuple(ws)}: x is [..., K], w [N, K]"
+    bf16 = torch.bfloat16
+    assert x.dtype == bf16 and w.dtype == bf16, f"linear_act takes bfloat16, got {x.dtype} and {w.dtype}"
+    if bias is not None:
+        assert bias.shape == ws[:1], f"bias {tuple(bias.shape)}: one value per row of w"
+        assert bias.dtype == bf16, f"linear_act takes bfloat16, got a bias of {bias.dtype}"
+    if residual is not None:
+        assert residual.shape == xs[:-1] + ws[:1], f"residual {tuple(residual.shape)}: the shape of the result"
+        assert residual.dtype == bf16, f"linear_act takes bfloat16, got a residual of {residual.dtype}"
+    return act
 
 
 def _ld(t: Tensor) -> int:
@@ -89,7 +103,10 @@ def _ld(t: Tensor) -> int:
 
 def _matrix(t: Tensor) -> Tensor:
     """[..., K] as a matrix whose rows are contiguous and do not overlap: a view where there is one."""
-    t = t if t.ndim == 2 else t.reshape(-1, t.shape[-1])
+    if t.ndim != 2:
+        t = t.reshape(-1, t.shape[-1])
+    if t.is_contiguous():
+        return t
     return t if (t.stride(1) == 1 or t.shape[1] == 1) and _ld(t) >= t.shape[1] else t.contiguous()
 
 
@@ -98,7 +115,7 @@ def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | No
     assert act or not keep_pre, "keep_pre: without an activation the backward needs no pre-activation"
     gpu = _same_gpu(x, w, bias, residual)
     N, K = w.shape
-    out = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
+    out = x.new_empty(x.shape[:-1] + (N,))
     pre = torch.empty_like(out) if keep_pre else None
     if out.numel() == 0:
         return out, pre
@@ -108,8 +125,9 @@ def _linear_fwd(x: Tensor, w: Tensor, bias: Tensor | None, residual: Tensor | No
     if bias is not None and (bias.stride(0) != 1 or bias.data_ptr() % 16):
         bias = bias.clone(memory_format=torch.contiguous_format)
     res = None if residual is None else _matrix(residual)
-    _launch(gpu, "ngpt_linear_act_fwd", _p(xr), _ld(xr), _p(wr), _ld(wr), _p(bias), _p(res), 0 if res is None else _ld(res), xr.shape[0], N, K, act,
-            _p(out), _p(pre))
+    _launch(gpu, "ngpt_linear_act_fwd", xr.data_ptr(), _ld(xr), wr.data_ptr(), _ld(wr), None if bias is None else bias.data_ptr(),
+            None if res is None else res.data_ptr(), 0 if res is None else _ld(res), xr.shape[0], N, K, act, out.data_ptr(),
+            None if pre is None else pre.data_ptr())
     return out, pre
 
 
@@ -221,16 +239,17 @@ def linear_act(x: Tensor, w: Tensor, bias: Tensor | None = None, residual: Tenso
 # qk_norm_rope
 
 def _rope_shapes(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Tensor | None, q_weight: Tensor | None, k_weight: Tensor | None) -> None:
-    assert q.ndim in (3, 4) and k.ndim == q.ndim and q.shape[:-2] == k.shape[:-2] and q.shape[-1] == k.shape[-1], (
-        f"q {tuple(q.shape)} and k {tuple(k.shape)}: [T, H, D] or [B, T, H, D] with the same tokens and head size")
-    assert q.dtype in _DTYPES and k.dtype == q.dtype, f"q {q.dtype} and k {k.dtype}: both bfloat16 or both float32"
+    qs, ks, dtype = q.shape, k.shape, q.dtype
+    assert len(qs) in (3, 4) and len(ks) == len(qs) and qs[:-2] == ks[:-2] and qs[-1] == ks[-1], (
+        f"q {tuple(qs)} and k {tuple(ks)}: [T, H, D] or [B, T, H, D] with the same tokens and head size")
+    assert dtype in _DTYPES and k.dtype == dtype, f"q {dtype} and k {k.dtype}: both bfloat16 or both float32"
     assert cos.ndim == 2 and cos.shape == sin.shape and cos.dtype == sin.dtype and cos.dtype in _DTYPES, (
         "cos and sin: [positions, rotated / 2], both bfloat16 or both float32")
-    tokens = q.shape[:-2]
-    assert positions is None or (positions.dtype in (torch.int32, torch.int64) and tuple(positions.shape) in (tuple(tokens), (tokens[-1],))), (
-        f"positions: int32 or int64, of shape {tuple(tokens)} or {(tokens[-1],)}")
+    if positions is not None:
+        assert positions.dtype in (torch.int32, torch.int64) and (positions.shape == qs[:-2] or positions.shape == qs[-3:-2]), (
+            f"positions: int32 or int64, of shape {tuple(qs[:-2])} or {tuple(qs[-3:-2])}")
     for w in (q_weight, k_weight):
-        assert w is None or (w.shape == (q.shape[-1],) and w.dtype == q.dtype), "weights: one value per head element, in the heads' type"
+        assert w is None or (w.shape == qs[-1:] and w.dtype == dtype), "weights: one value per head element, in the heads' type"
 
 
 def _heads(t: Tensor) -> Tensor:
@@ -268,8 +287,7 @@ def _rope_common(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved
 def _rope_fwd(q, k, cos, sin, positions, q_weight, k_weight, eps, interleaved) -> tuple[Tensor, Tensor]:
     _rope_shapes(q, k, cos, sin, positions, q_weight, k_weight)
     gpu = _same_gpu(q, k, cos, sin, positions, q_weight, k_weight)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
     if q.numel() == 0 and k.numel() == 0:
         return q_out, k_out
     q, k = _heads(q), _heads(k)
@@ -282,8 +300,7 @@ def _rope_bwd(dq_out, dk_out, q, k, cos, sin, positions, q_weight, k_weight, eps
     """-> dq, dk, dq_weight or None, dk_weight or None"""
     gpu = _same_gpu(q, k, cos, sin, positions, q_weight, k_weight, dq_out, dk_out)
     assert dq_out.shape == q.shape and dk_out.shape == k.shape and dq_out.dtype == q.dtype and dk_out.dtype == k.dtype
-    dq = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    dk = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    dq, dk = q.new_empty(q.shape), k.new_empty(k.shape)
     dqw = torch.empty_like(q_weight, memory_format=torch.contiguous_format) if need_dqw else None
     dkw = torch.empty_like(k_weight, memory_format=torch.contiguous_format) if need_dkw else None
     if q.numel() == 0 and k.numel() == 0:
