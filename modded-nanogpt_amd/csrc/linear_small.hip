@@ -298,12 +298,14 @@ int linear_mid(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_
     std::integral_constant<int, 2> c2;
     std::integral_constant<int, 4> c4;
     auto tiles = [&](int b) { return (int64_t)((o.N + b - 1) / b) * ((o.M + b - 1) / b); };
-    if (tiles(128) >= 2 * (int64_t)cus) return go(c2, c1);
-    // tiles of 64: about sixteen waves a compute unit
+    // one 128 x 128 tile for every compute unit (1024 x 1024 -> 4096: 16.3 us, tiles of 64: 17.9; 2048 x 4096 -> 1024, half as many: 49 against 34)
+    if (tiles(128) >= cus) return go(c2, c1);
+    // Tiles of 64: a contraction in two where there are few (1024 x 1024 -> 1024: 7.1 us, in one piece 8.0, in four 7.5), in four where it is long
+    // as well (1024 x 4096 -> 1024: 18.9 us, in two 20.3, in one piece 27.6).
     const int64_t t64 = tiles(64);
     const int steps = (K + 63) / 64;
     if (t64 >= 3 * (int64_t)cus || steps < 4) return go(c1, c1);
-    if (t64 > cus || steps < 8) return go(c1, c2);
+    if (t64 > cus || steps < 32) return go(c1, c2);
     return go(c1, c4);
 }
 
