@@ -3,10 +3,12 @@ or a call fails, an exception is raised -- there is no fallback implementation."
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import pathlib
 from ctypes import c_char_p, c_float, c_int, c_int64, c_void_p
 
 LIB_PATH = pathlib.Path(__file__).resolve().parent / "lib" / "libngpt_fp8.so"
+BINDING_PATH = LIB_PATH.with_name("_ngpt_torch.so")
 # the same sources compiled with -DNGPT_BENCH_BUILD: adds the timing aids that measurements use and nothing else needs
 BENCH_LIB_PATH = LIB_PATH.with_name("libngpt_fp8_bench.so")
 BENCH_SIGNATURES = {
@@ -88,6 +90,7 @@ SIGNATURES = {
 
 _lib = None
 _bench_lib = None
+_binding = None
 
 
 class NgptError(RuntimeError):
@@ -108,6 +111,20 @@ def load() -> ctypes.CDLL:
             fn.restype, fn.argtypes = res, args
         _lib = lib
     return _lib
+
+
+def load_torch():
+    """The torch binding (lib/_ngpt_torch.so), a Python module; raises if it is not built."""
+    global _binding
+    if _binding is None:
+        load()
+        if not BINDING_PATH.exists():
+            raise NgptError(f"{BINDING_PATH} is not built; run `python -m modded_nanogpt_amd.build` (there is no fallback path)")
+        spec = importlib.util.spec_from_file_location("_ngpt_torch", BINDING_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        _binding = module
+    return _binding
 
 
 def load_bench() -> ctypes.CDLL:

@@ -1,4 +1,4 @@
-"""Builds libngpt_fp8.so (all HIP kernels + the C ABI) for gfx950 with hipcc, in-tree.
+"""Builds libngpt_fp8.so (all HIP kernels + the C ABI) for gfx950 with hipcc, in-tree, and the host-side torch binding beside it.
 
     python -m modded_nanogpt_amd.build          # from the repository root
 
@@ -19,6 +19,7 @@ PKG = pathlib.Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB_DIR = PKG / "lib"
 LIB_PATH = LIB_DIR / "libngpt_fp8.so"
+BINDING_PATH = LIB_DIR / "_ngpt_torch.so"             # torch_binding.cpp: host code that calls the library for torch tensors
 BENCH_LIB_PATH = LIB_DIR / "libngpt_fp8_bench.so"     # + the timing aids behind NGPT_BENCH_BUILD, for measurements only
 SOURCES = ["gemm_api.hip", "quant.hip", "ce.hip", "mlp_aux.hip", "linear.hip", "linear_small.hip", "qk_rope.hip", "distill.hip", "bench_kernels.hip"]   # the last one is empty without NGPT_BENCH_BUILD
 
@@ -50,6 +51,24 @@ def _run(cmd: list[str], verbose: bool) -> None:
         print(err, file=sys.stderr)
 
 
+def _binding_commands(obj: str, lib_dir: str) -> tuple[list[str], list[str]]:
+    """Commands that compile and link the torch binding (host code only)."""
+    import sysconfig
+
+    import torch
+    from torch.utils.cpp_extension import include_paths, library_paths
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if not cxx:
+        raise RuntimeError("no C++ compiler for the torch binding")
+    rocm = pathlib.Path(hipcc_path()).resolve().parent.parent
+    compile_ = [cxx, "-O2", "-std=c++17", "-fPIC", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                *[f"-isystem{p}" for p in include_paths()], f"-isystem{rocm / 'include'}", "-isystem/opt/rocm/include",
+                f"-I{sysconfig.get_paths()['include']}", "-c", "-o", obj, str(CSRC / "torch_binding.cpp")]
+    link = [cxx, "-shared", "-o", str(BINDING_PATH) + ".tmp", obj, f"-L{lib_dir}", "-l:libngpt_fp8.so", *[f"-L{p}" for p in library_paths()],
+            "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_hip", "-ltorch_python", "-Wl,-rpath,$ORIGIN"]
+    return compile_, link
+
+
 def build(verbose: bool = True, bench: bool = False) -> pathlib.Path:
     """Compile every HIP source into one shared library; always recompiles.  `bench`: the measurement build."""
     LIB_DIR.mkdir(exist_ok=True)
@@ -59,11 +78,16 @@ def build(verbose: bool = True, bench: bool = False) -> pathlib.Path:
     flags = [*[f for f in HIPCC_FLAGS if f != "-shared"], *(["-DNGPT_BENCH_BUILD"] if bench else []), "-I", str(PKG.parent / "include")]
     with tempfile.TemporaryDirectory() as objdir:
         # one object a source, compiled side by side, then one link
+        binding = None if bench else _binding_commands(str(pathlib.Path(objdir) / "torch_binding.o"), str(LIB_DIR))
         objs = [str(pathlib.Path(objdir) / (pathlib.Path(s).stem + ".o")) for s in srcs]
-        with ThreadPoolExecutor(max_workers=min(len(srcs), os.cpu_count() or 1, 8)) as pool:
-            list(pool.map(lambda so: _run([hipcc_path(), *flags, "-c", "-o", so[1], so[0]], verbose), zip(srcs, objs)))
+        jobs = [[hipcc_path(), *flags, "-c", "-o", o, c] for c, o in zip(srcs, objs)] + ([binding[0]] if binding else [])
+        with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 1, 8)) as pool:
+            list(pool.map(lambda job: _run(job, verbose), jobs))
         _run([hipcc_path(), *HIPCC_FLAGS, "-o", str(tmp), *objs], verbose)
-    os.replace(tmp, out)
+        os.replace(tmp, out)
+        if binding:
+            _run(binding[1], verbose)
+            os.replace(str(BINDING_PATH) + ".tmp", BINDING_PATH)
     return out
 
 
