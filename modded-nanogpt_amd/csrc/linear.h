@@ -61,24 +61,36 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float lo16(int w) { return __uint_as_float((uint32_t)w << 16); }
 __device__ __forceinline__ float hi16(int w) { return __uint_as_float((uint32_t)w & 0xffff0000u); }
 
-// 8 consecutive bf16 of a row, `n` > 0 of which exist: 16 bytes at any address (gfx950 takes unaligned global accesses), a row's last values
-// one by one.  That is a loop on purpose: the compiler stops inlining into a kernel of many basic blocks, and a GEMM's state then lives in
-// scratch memory.
-__device__ __forceinline__ v4i load_any(const uint16_t* p, int n) {
+// Values i .. i + 7 of a row of `len` (zeros behind its end; 0 <= i), 16 bytes at any address: gfx950 takes unaligned global accesses.  The
+// row's last, incomplete piece is loaded so that it ends with the row and shifted down; only rows of less than 8 values go one by one.
+__device__ __forceinline__ v4i load_row8(const uint16_t* row, int i, int len) {
     v4i w = {0, 0, 0, 0};
-    if (n >= 8) {
-        __builtin_memcpy(&w, p, 16);
+    if (i + 8 <= len) {
+        __builtin_memcpy(&w, row + i, 16);
+        return w;
+    }
+    if (i >= len) return w;
+    if (len >= 8) {
+        const int s = i + 8 - len;
+        __builtin_memcpy(&w, row + (len - 8), 16);
+        if (s & 4) w = (v4i){w.z, w.w, 0, 0};
+        if (s & 2) w = (v4i){w.y, w.z, w.w, 0};
+        if (s & 1)
+            w = (v4i){(int)__builtin_amdgcn_alignbit((uint32_t)w.y, (uint32_t)w.x, 16), (int)__builtin_amdgcn_alignbit((uint32_t)w.z, (uint32_t)w.y, 16),
+                      (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16), (int)((uint32_t)w.w >> 16)};
         return w;
     }
 #pragma unroll 1
-    for (int i = n - 1; i >= 0; --i) {
+    for (int e = min(len - i, 8) - 1; e >= 0; --e) {
         w.w = (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16);
         w.z = (int)__builtin_amdgcn_alignbit((uint32_t)w.z, (uint32_t)w.y, 16);
         w.y = (int)__builtin_amdgcn_alignbit((uint32_t)w.y, (uint32_t)w.x, 16);
-        w.x = (int)(((uint32_t)w.x << 16) | (uint32_t)p[i]);
+        w.x = (int)(((uint32_t)w.x << 16) | (uint32_t)row[i + e]);
     }
     return w;
 }
+// The first `n` > 0 of 8 values (a loop on purpose: the compiler stops inlining into a kernel of many basic blocks, and a GEMM's state then
+// lives in scratch memory).
 __device__ __forceinline__ void store_any(uint16_t* p, v4i w, int n) {
     if (n >= 8) {
         __builtin_memcpy(p, &w, 16);
@@ -163,9 +175,8 @@ __device__ __forceinline__ void linear_epilogue(const LinearOut& o, v16f (&acc)[
             const int row = RPI * k + rd_row, m = m0 + tn * 32 + row, left = N - f;
             uint8_t* at = stage + swz(row, rd_chunk);
             if (m < o.M && left > 0) {
-                const int64_t i = (int64_t)m * ld + f;
-                if (to) store_any(to + i, *(const v4i*)at, left);
-                else *(v4i*)at = load_any(from + i, left);
+                if (to) store_any(to + (int64_t)m * ld + f, *(const v4i*)at, left);
+                else *(v4i*)at = load_row8(from + (int64_t)m * ld, f, N);
             }
         }
     };

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(256) void pad_copy_kernel(const uint16_t* __restric
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256) {
         const int r = (int)(i / c8), c = (int)(i - (int64_t)r * c8) * 8;
         v4i w = {0, 0, 0, 0};
-        if (r < rows && c < cols) w = load_any(src + (int64_t)r * ld + c, cols - c);
+        if (r < rows && c < cols) w = load_row8(src + (int64_t)r * ld, c, cols);
         *(v4i*)(dst + i * 8) = w;
     }
 }
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(256) void transpose_pad_kernel(const uint16_t* __re
     for (int i = 0; i < 2; ++i) {
         const int r = (t >> 3) + 32 * i, c = (t & 7) * 8, left = cols - c0 - c;
         v4i w = {0, 0, 0, 0};
-        if (r0 + r < rows && left > 0) w = load_any(src + (int64_t)(r0 + r) * ld + c0 + c, left);
+        if (r0 + r < rows && left > 0) w = load_row8(src + (int64_t)(r0 + r) * ld, c0 + c, cols);
 #pragma unroll
         for (int e = 0; e < 4; ++e) *(uint32_t*)&tile[r][c + 2 * e] = (uint32_t)w[e];
     }
@@ -103,7 +103,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restric
         for (int r = blockIdx.y * kRowLanes + rt; r < rows_p; r += gridDim.y * kRowLanes) {
             v4i g = {0, 0, 0, 0}, o = {0, 0, 0, 0};
             if (r < M && c < N) {
-                g = load_any(dout + (int64_t)r * N + c, N - c);
+                g = load_row8(dout + (int64_t)r * N, c, N);
                 if constexpr (ACT == NGPT_ACT_NONE) {
                     o = g;
 #pragma unroll
@@ -112,7 +112,7 @@ __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restric
                         sum[2 * i + 1] += hi16(g[i]);
                     }
                 } else {
-                    const v4i z = load_any(pre + (int64_t)r * N + c, N - c);
+                    const v4i z = load_row8(pre + (int64_t)r * N, c, N);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float d0 = lo16(g[i]) * act_slope<ACT>(lo16(z[i])), d1 = hi16(g[i]) * act_slope<ACT>(hi16(z[i]));

@@ -9,9 +9,6 @@
 namespace ngpt {
 namespace {
 
-// values k .. k + 7 of a row of K; zeros behind its end
-__device__ __forceinline__ v4i load_k8(const uint16_t* row, int k, int K) { return k < K ? load_any(row + k, K - k) : (v4i){0, 0, 0, 0}; }
-
 template <class F>
 __device__ __forceinline__ void act_switch(int act, F&& f) {      // wave-uniform
     switch (act) {
@@ -47,20 +44,22 @@ __global__ __launch_bounds__(1024) void linear_few_kernel(LinearOut o, const uin
 #pragma unroll
         for (int j = 0; j < MT; ++j) acc[i][j] = (v4f){0, 0, 0, 0};
     const int units = (K + 63) / 64;
-    for (int u0 = wave; u0 < units; u0 += waves * U) {
-        v4i a[U][2][FT], b[U][2][MT];
+    // U units a pass, all of whose loads are in flight together; the last units, one of which may end inside the contraction, one by one
+    auto pass = [&](int u0, auto count, auto load) {
+        constexpr int C = decltype(count)::value;
+        v4i a[C][2][FT], b[C][2][MT];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < C; ++u)
 #pragma unroll
             for (int s = 0; s < 2; ++s) {
-                const int k = (u0 + u * waves) * 64 + s * 32 + q * 8;      // past the end: zeros
+                const int k = (u0 + u * waves) * 64 + s * 32 + q * 8;
 #pragma unroll
-                for (int i = 0; i < FT; ++i) a[u][s][i] = load_k8(wr[i], k, K);
+                for (int i = 0; i < FT; ++i) a[u][s][i] = load(wr[i], k);
 #pragma unroll
-                for (int j = 0; j < MT; ++j) b[u][s][j] = load_k8(xr[j], k, K);
+                for (int j = 0; j < MT; ++j) b[u][s][j] = load(xr[j], k);
             }
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+        for (int u = 0; u < C; ++u)
 #pragma unroll
             for (int s = 0; s < 2; ++s)
 #pragma unroll
@@ -69,7 +68,17 @@ __global__ __launch_bounds__(1024) void linear_few_kernel(LinearOut o, const uin
                     for (int j = 0; j < MT; ++j)
                         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a[u][s][i]), __builtin_bit_cast(v8bf, b[u][s][j]),
                                                                             acc[i][j], 0, 0, 0);
-    }
+    };
+    auto whole = [](const uint16_t* row, int k) {
+        v4i v;
+        __builtin_memcpy(&v, row + k, 16);
+        return v;
+    };
+    std::integral_constant<int, 1> one;
+    int u0 = wave;
+    for (; (u0 + (U - 1) * waves + 1) * 64 <= K; u0 += waves * U) pass(u0, std::integral_constant<int, U>{}, whole);
+    for (; (u0 + 1) * 64 <= K; u0 += waves) pass(u0, one, whole);
+    if (u0 < units) pass(u0, one, [K](const uint16_t* row, int k) { return load_row8(row, k, K); });
 #pragma unroll
     for (int i = 0; i < FT; ++i)
 #pragma unroll
@@ -162,7 +171,7 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : 2) void linear_mid_kernel(L
             for (int i = 0; i < Cfg::LOADS; ++i) __builtin_memcpy(&reg[i], (i < Cfg::LOADS / 2 ? wt : xt) + off[i] + k, 16);
         } else {
 #pragma unroll
-            for (int i = 0; i < Cfg::LOADS; ++i) reg[i] = load_k8((i < Cfg::LOADS / 2 ? wt : xt) + off[i], k, K);
+            for (int i = 0; i < Cfg::LOADS; ++i) reg[i] = load_row8((i < Cfg::LOADS / 2 ? wt : xt) + off[i], k, K);
         }
     };
     auto put = [&](int stage, const v4i (&reg)[Cfg::LOADS]) {
