@@ -61,25 +61,23 @@ typedef unsigned int u32x4 __attribute__((ext_vector_type(4)));
 __device__ __forceinline__ float lo16(int w) { return __uint_as_float((uint32_t)w << 16); }
 __device__ __forceinline__ float hi16(int w) { return __uint_as_float((uint32_t)w & 0xffff0000u); }
 
-// Values i .. i + 7 of a row of `len` (zeros behind its end; 0 <= i), 16 bytes at any address: gfx950 takes unaligned global accesses.  The
-// row's last, incomplete piece is loaded so that it ends with the row and shifted down; only rows of less than 8 values go one by one.
-__device__ __forceinline__ v4i load_row8(const uint16_t* row, int i, int len) {
+// Values i .. i + 7 of a row of `len` (zeros behind its end; 0 <= i), 16 bytes at any address: gfx950 takes unaligned global accesses.
+// Of a row of 8 values and more, without a branch: the piece is loaded so that it ends with the row at the latest, and shifted down.
+__device__ __forceinline__ v4i load_row8_end(const uint16_t* row, int i, int len) {
+    const int at = min(i, len - 8), s = i - at;
+    v4i w;
+    __builtin_memcpy(&w, row + at, 16);
+    if (s & 4) w = (v4i){w.z, w.w, 0, 0};
+    if (s & 2) w = (v4i){w.y, w.z, w.w, 0};
+    if (s & 1)
+        w = (v4i){(int)__builtin_amdgcn_alignbit((uint32_t)w.y, (uint32_t)w.x, 16), (int)__builtin_amdgcn_alignbit((uint32_t)w.z, (uint32_t)w.y, 16),
+                  (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16), (int)((uint32_t)w.w >> 16)};
+    if (s >= 8) w = (v4i){0, 0, 0, 0};
+    return w;
+}
+// of a row of any length, value by value
+__device__ __forceinline__ v4i load_row8_short(const uint16_t* row, int i, int len) {
     v4i w = {0, 0, 0, 0};
-    if (i + 8 <= len) {
-        __builtin_memcpy(&w, row + i, 16);
-        return w;
-    }
-    if (i >= len) return w;
-    if (len >= 8) {
-        const int s = i + 8 - len;
-        __builtin_memcpy(&w, row + (len - 8), 16);
-        if (s & 4) w = (v4i){w.z, w.w, 0, 0};
-        if (s & 2) w = (v4i){w.y, w.z, w.w, 0};
-        if (s & 1)
-            w = (v4i){(int)__builtin_amdgcn_alignbit((uint32_t)w.y, (uint32_t)w.x, 16), (int)__builtin_amdgcn_alignbit((uint32_t)w.z, (uint32_t)w.y, 16),
-                      (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16), (int)((uint32_t)w.w >> 16)};
-        return w;
-    }
 #pragma unroll 1
     for (int e = min(len - i, 8) - 1; e >= 0; --e) {
         w.w = (int)__builtin_amdgcn_alignbit((uint32_t)w.w, (uint32_t)w.z, 16);
@@ -88,6 +86,16 @@ __device__ __forceinline__ v4i load_row8(const uint16_t* row, int i, int len) {
         w.x = (int)(((uint32_t)w.x << 16) | (uint32_t)row[i + e]);
     }
     return w;
+}
+__device__ __forceinline__ v4i load_row8(const uint16_t* row, int i, int len) {
+    v4i w = {0, 0, 0, 0};
+    if (i + 8 <= len) {
+        __builtin_memcpy(&w, row + i, 16);
+        return w;
+    }
+    if (i >= len) return w;
+    if (len >= 8) return load_row8_end(row, i, len);
+    return load_row8_short(row, i, len);
 }
 // The first `n` > 0 of 8 values (a loop on purpose: the compiler stops inlining into a kernel of many basic blocks, and a GEMM's state then
 // lives in scratch memory).

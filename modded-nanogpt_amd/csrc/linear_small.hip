@@ -21,74 +21,105 @@ __device__ __forceinline__ void act_switch(int act, F&& f) {      // wave-unifor
 }
 
 // ---------------------------------------------------------------------------------------------- few rows
+// A 4 x 4 exchange in every quad of lanes: register j of lane p takes what lane j of its quad holds in register p.
+__device__ __forceinline__ void quad_transpose(v4i (&v)[4], bool odd, bool high) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+        auto swap = [&](auto perm, bool up, int& lo, int& hi) {
+            constexpr int P = decltype(perm)::value;
+            const int from_hi = __builtin_amdgcn_update_dpp(0, hi, P, 0xf, 0xf, true), from_lo = __builtin_amdgcn_update_dpp(0, lo, P, 0xf, 0xf, true);
+            const int l = up ? from_hi : lo, h = up ? hi : from_lo;
+            lo = l;
+            hi = h;
+        };
+        int t[4] = {v[0][e], v[1][e], v[2][e], v[3][e]};
+        std::integral_constant<int, 0xB1> one;      // lane ^ 1
+        std::integral_constant<int, 0x4E> two;      // lane ^ 2
+        swap(one, odd, t[0], t[1]);
+        swap(one, odd, t[2], t[3]);
+        swap(two, high, t[0], t[2]);
+        swap(two, high, t[1], t[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j][e] = t[j];
+    }
+}
+
 // Every weight is read once and used for at most 32 rows: the bound is the weights' way from memory, and for one token the launch and one
-// round trip.  A workgroup owns 16 FT features; its waves share the contraction in units of 64 values (a line of every weight row), with all
-// loads of U units in flight, multiply on 16x16x32 matrix instructions (rows past M repeat the last and are dropped) and add up through LDS
-// in wave order.
+// round trip.  A workgroup owns 16 features; its waves share the contraction in units of 128 values, with all loads of U units in flight,
+// multiply on 16x16x32 matrix instructions (rows past M repeat the last and are dropped) and add up through LDS in wave order.
 // Matrix instruction: lane l, q = l / 16: A row / B column l % 16, contraction 8 q .. 8 q + 7; D column l % 16, rows 4 q .. 4 q + 3.
-template <int FT, int MT, int U>
+// Loaded in that order the four lanes of a quad would read from four rows, and the load unit takes such an instruction at about 45 clocks.  So
+// load j reads rows j, 4 + j, 8 + j and 12 + j with the quad's lanes side by side, and the quads exchange in registers: lane (q, 4 a + p) then
+// holds of row 4 a + p the piece 4 q + j of the unit in register j, for both operands.
+// 12 x 4096 -> 1024: 7.0 us (8.8 without the exchange), 16 x 2048 -> 2048: 4.1 (6.0), 32 x 4096 -> 1024: 7.4 (12.9), 1 x 1024 -> 4096: 4.1, of which
+// an empty launch is about 2.5; rows at odd addresses, 12 x 4095 -> 1023: 10.8.  Only N / 16 workgroups work, so a narrow result with a long
+// contraction stays furthest from the memory's rate.  (Groups of 8 or 4 features: no shorter at any of these, 16 x 2048 -> 2048 9.7 with 4.)
+template <int MT, int U>
 __global__ __launch_bounds__(1024) void linear_few_kernel(LinearOut o, const uint16_t* __restrict__ x, int64_t ldx, const uint16_t* __restrict__ w,
                                                           int64_t ldw, int K, int act) {
-    extern __shared__ __attribute__((aligned(16))) v4f part[];      // [wave][FT][MT][lane]
+    extern __shared__ __attribute__((aligned(16))) v4f part[];      // [wave][MT][lane]
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int r = lane & 15, q = lane >> 4;
-    const int f0 = blockIdx.x * 16 * FT;
-    const uint16_t *wr[FT], *xr[MT];
+    const bool odd = lane & 1, high = lane & 2;
+    const int f0 = blockIdx.x * 16, row0 = r & 12, k0 = 32 * q + 8 * (lane & 3);
+    const uint16_t *wr[4], *xr[MT][4];
 #pragma unroll
-    for (int i = 0; i < FT; ++i) wr[i] = w + (int64_t)min(f0 + 16 * i + r, o.N - 1) * ldw;
+    for (int j = 0; j < 4; ++j) {
+        wr[j] = w + (int64_t)min(f0 + row0 + j, o.N - 1) * ldw + k0;
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xr[i] = x + (int64_t)min(16 * i + r, o.M - 1) * ldx;
-    v4f acc[FT][MT];
+        for (int m = 0; m < MT; ++m) xr[m][j] = x + (int64_t)min(16 * m + row0 + j, o.M - 1) * ldx + k0;
+    }
+    v4f acc[MT];
 #pragma unroll
-    for (int i = 0; i < FT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = (v4f){0, 0, 0, 0};
-    const int units = (K + 63) / 64;
+    for (int m = 0; m < MT; ++m) acc[m] = (v4f){0, 0, 0, 0};
     // U units a pass, all of whose loads are in flight together; the last units, one of which may end inside the contraction, one by one
     auto pass = [&](int u0, auto count, auto load) {
         constexpr int C = decltype(count)::value;
-        v4i a[C][2][FT], b[C][2][MT];
+        v4i a[C][4], b[C][MT][4];
 #pragma unroll
-        for (int u = 0; u < C; ++u)
+        for (int u = 0; u < C; ++u) {
+            const int k = (u0 + u * waves) * 128;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                const int k = (u0 + u * waves) * 64 + s * 32 + q * 8;
+            for (int j = 0; j < 4; ++j) a[u][j] = load(wr[j], k);
 #pragma unroll
-                for (int i = 0; i < FT; ++i) a[u][s][i] = load(wr[i], k);
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-                for (int j = 0; j < MT; ++j) b[u][s][j] = load(xr[j], k);
+                for (int j = 0; j < 4; ++j) b[u][m][j] = load(xr[m][j], k);
+        }
+        __builtin_amdgcn_sched_barrier(0);      // first every load of the pass, then the exchanges that wait for them
+#pragma unroll
+        for (int u = 0; u < C; ++u) {
+            quad_transpose(a[u], odd, high);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+                quad_transpose(b[u][m], odd, high);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a[u][j]), __builtin_bit_cast(v8bf, b[u][m][j]), acc[m],
+                                                                     0, 0, 0);
             }
-#pragma unroll
-        for (int u = 0; u < C; ++u)
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int i = 0; i < FT; ++i)
-#pragma unroll
-                    for (int j = 0; j < MT; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a[u][s][i]), __builtin_bit_cast(v8bf, b[u][s][j]),
-                                                                            acc[i][j], 0, 0, 0);
+        }
     };
-    auto whole = [](const uint16_t* row, int k) {
+    auto whole = [](const uint16_t* at, int k) {
         v4i v;
-        __builtin_memcpy(&v, row + k, 16);
+        __builtin_memcpy(&v, at + k, 16);
         return v;
     };
     std::integral_constant<int, 1> one;
     int u0 = wave;
-    for (; (u0 + (U - 1) * waves + 1) * 64 <= K; u0 += waves * U) pass(u0, std::integral_constant<int, U>{}, whole);
-    for (; (u0 + 1) * 64 <= K; u0 += waves) pass(u0, one, whole);
-    if (u0 < units) pass(u0, one, [K](const uint16_t* row, int k) { return load_row8(row, k, K); });
+    for (; (u0 + (U - 1) * waves + 1) * 128 <= K; u0 += waves * U) pass(u0, std::integral_constant<int, U>{}, whole);
+    for (; (u0 + 1) * 128 <= K; u0 += waves) pass(u0, one, whole);
+    if (u0 * 128 < K) {
+        if (K >= 8) pass(u0, one, [K, k0](const uint16_t* at, int k) { return load_row8_end(at - k0, k0 + k, K); });
+        else pass(u0, one, [K, k0](const uint16_t* at, int k) { return load_row8_short(at - k0, k0 + k, K); });
+    }
 #pragma unroll
-    for (int i = 0; i < FT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) part[((wave * FT + i) * MT + j) * 64 + lane] = acc[i][j];
+    for (int m = 0; m < MT; ++m) part[(wave * MT + m) * 64 + lane] = acc[m];
     __syncthreads();
-    for (int t = wave; t < FT * MT; t += waves) {
+    for (int t = wave; t < MT; t += waves) {
         v4f z = part[t * 64 + lane];
-        for (int p = 1; p < waves; ++p) z += part[(p * FT * MT + t) * 64 + lane];
-        const int i = t / MT, j = t % MT;
-        const int m = 16 * j + r, f = f0 + 16 * i + 4 * q, left = o.N - f;
+        for (int p = 1; p < waves; ++p) z += part[(p * MT + t) * 64 + lane];
+        const int m = 16 * t + r, f = f0 + 4 * q, left = o.N - f;
         if (m >= o.M || left <= 0) continue;
         const int64_t at = (int64_t)m * o.N + f;
         float y[4];
@@ -265,22 +296,21 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : 2) void linear_mid_kernel(L
 int linear_few(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int K, int act, hipStream_t st) {
     const int cus = num_cus();
     if (cus <= 0) return fail(NGPT_EINVAL, "no HIP device");
-    auto go = [&](auto ft, auto mt, auto u) {
-        constexpr int FT = decltype(ft)::value, MT = decltype(mt)::value, U = decltype(u)::value;
-        const int groups = (o.N + 16 * FT - 1) / (16 * FT), units = (K + 63) / 64;
+    auto go = [&](auto mt, auto u) {
+        constexpr int MT = decltype(mt)::value, U = decltype(u)::value;
+        const int groups = (o.N + 15) / 16, units = (K + 127) / 128;
         // waves that share a group's contraction: as many as there are units for, fewer where the groups alone fill the compute units
         int waves = groups <= cus ? 16 : (groups <= 2 * cus ? 8 : 4);
         while (waves > 1 && waves > units) waves /= 2;
-        const int lds = waves * FT * MT * 1024;
-        static_assert(16 * FT * MT * 1024 <= 65536, "fits without asking for more");
-        linear_few_kernel<FT, MT, U><<<groups, 64 * waves, lds, st>>>(o, x, ldx, w, ldw, K, act);
+        const int lds = waves * MT * 1024;
+        static_assert(16 * MT * 1024 <= 65536, "fits without asking for more");
+        linear_few_kernel<MT, U><<<groups, 64 * waves, lds, st>>>(o, x, ldx, w, ldw, K, act);
         return check_launch("linear_few_kernel");
     };
     std::integral_constant<int, 1> c1;
     std::integral_constant<int, 2> c2;
-    std::integral_constant<int, 4> c4;
-    if (o.M <= 16) return go(c1, c1, c4);
-    return go(c1, c2, c2);
+    if (o.M <= 16) return go(c1, c2);
+    return go(c2, c1);
 }
 
 int linear_mid(const LinearOut& o, const uint16_t* x, int64_t ldx, const uint16_t* w, int64_t ldw, int K, int act, hipStream_t st) {
