@@ -46,12 +46,27 @@ def _plain(*tensors: Tensor | None) -> bool:
 
 
 def _rows(t: Tensor | None) -> Tensor | None:
-    """[..., K] whose rows are contiguous and do not overlap: itself, or a copy."""
-    if t is None or t.is_contiguous():
+    """[..., K] whose rows are contiguous, evenly spaced and do not overlap: itself, or a copy."""
+    if t is None or t.is_contiguous() or t.ndim == 0:
         return t
-    if t.ndim == 2 and (t.stride(1) == 1 or t.shape[1] == 1) and (t.stride(0) >= t.shape[1] or t.shape[0] == 1):
+    if (t.ndim > 1 and (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-2) >= t.shape[-1]
+            and all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.ndim - 2))):
         return t
     return t.contiguous()
+
+
+def _direct(*tensors: Tensor | None) -> bool:
+    """Memory that a kernel can be given: not the meta device, whose tensors take the registered operators."""
+    for t in tensors:
+        if t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise RuntimeError("nanogpt operators do not go through torch.func's transforms; use torch.autograd")
+    return not any(t is not None and t.is_meta for t in tensors)
+
+
+def _launched(out, what: str):
+    if out is None:
+        raise RuntimeError(f"{what}: the kernels cannot take these tensors (a dimension of 2^31 or more, no heads, or a tensor without memory of its own)")
+    return out
 
 
 def _contiguous(t: Tensor | None) -> Tensor | None:
@@ -153,9 +168,10 @@ def linear_act(x: Tensor, w: Tensor, bias: Tensor | None = None, residual: Tenso
             if out is not None:
                 return out
         act = _linear_shapes(x, w, bias, residual, activation)
-        _same_gpu(x, w, bias, residual)
-        if x.numel() and w.numel():
-            return _b().linear_act(*_linear_usable(x, w, bias, residual), act)
+        if _direct(x, w, bias, residual):
+            _same_gpu(x, w, bias, residual)
+            if x.numel() and w.numel():
+                return _launched(_b().linear_act(*_linear_usable(x, w, bias, residual), act), "linear_act")
     keep = activation != "none" and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias))
     return torch.ops.nanogpt.linear_act(x, w, bias, residual, activation, keep)[0]
 
@@ -190,7 +206,7 @@ def qk_norm_rope_op(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: T
     if q.numel() == 0 and k.numel() == 0:
         return q.new_empty(q.shape), k.new_empty(k.shape)
     with torch.no_grad():
-        return _b().qk_norm_rope(*_rope_usable(*tensors), eps, interleaved)
+        return _launched(_b().qk_norm_rope(*_rope_usable(*tensors), eps, interleaved), "qk_norm_rope")
 
 
 @qk_norm_rope_op.register_fake
@@ -252,11 +268,10 @@ def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Tens
         if out is not None:
             return out
         _rope_shapes(*tensors)
-        _same_gpu(*tensors)
-        if q.numel() or k.numel():
-            out = _b().qk_norm_rope(*_rope_usable(*tensors), eps, interleaved)
-            assert out is not None, f"q {tuple(q.shape)} and k {tuple(k.shape)}: no heads, or too many"
-            return out
+        if _direct(*tensors):
+            _same_gpu(*tensors)
+            if q.numel() or k.numel():
+                return _launched(_b().qk_norm_rope(*_rope_usable(*tensors), eps, interleaved), "qk_norm_rope")
     return torch.ops.nanogpt.qk_norm_rope(*tensors, eps, interleaved)
 
 
@@ -324,7 +339,7 @@ def distill_topk_fwd_bwd_op(logits: Tensor, ids: Tensor, teacher: Tensor, teache
     _same_gpu(*tensors)
     if _nothing_listed(logits, ids):
         return logits.new_zeros(logits.shape[0], dtype=torch.float32), logits.new_zeros(logits.shape)
-    return _b().distill_fused(*_distill_usable(*tensors), temperature, A, B, C, grad_scale)
+    return _launched(_b().distill_fused(*_distill_usable(*tensors), temperature, A, B, C, grad_scale), "distill_topk_fwd_bwd")
 
 
 @distill_topk_fwd_bwd_op.register_fake
@@ -378,9 +393,10 @@ def distill_topk(logits: Tensor, ids: Tensor, teacher: Tensor, teacher_lse: Tens
         if losses is not None:
             return losses
         _distill_shapes(*tensors)
-        _same_gpu(*tensors)
-        if not _nothing_listed(logits, ids):
-            return _b().distill_topk(*_distill_usable(*tensors), *params)
+        if _direct(*tensors):
+            _same_gpu(*tensors)
+            if not _nothing_listed(logits, ids):
+                return _launched(_b().distill_topk(*_distill_usable(*tensors), *params), "distill_topk")
     return torch.ops.nanogpt.distill_topk(*tensors, *params)[0]
 
 
@@ -396,7 +412,8 @@ def distill_topk_fwd_bwd(logits: Tensor, ids: Tensor, teacher: Tensor, teacher_l
         if out is not None:
             return out
         _distill_shapes(*tensors)
-        _same_gpu(*tensors)
-        if not _nothing_listed(logits, ids):
-            return _b().distill_fused(*(None if t is None else t.detach() for t in _distill_usable(*tensors)), *params)
+        if _direct(*tensors):
+            _same_gpu(*tensors)
+            if not _nothing_listed(logits, ids):
+                return _launched(_b().distill_fused(*_distill_usable(*tensors), *params), "distill_topk_fwd_bwd")
     return torch.ops.nanogpt.distill_topk_fwd_bwd(*tensors, *params)

@@ -8,6 +8,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/utils/pybind.h>
 #include "../../include/ngpt_fp8.h"
 
@@ -27,12 +28,17 @@ void check(int code, const char* what) {
     if (code != 0) TORCH_CHECK(false, what, " failed with code ", code, ": ", ngpt_last_error());
 }
 
-bool on_gpu(const Tensor& t, const Tensor& like) { return !t.defined() || (t.is_cuda() && t.device() == like.device()); }
-bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
+// Memory on that GPU (the wrappers of torch.func have none).
+bool on_gpu(const Tensor& t, const Tensor& like) { return !t.defined() || (t.is_cuda() && t.has_storage() && t.device() == like.device()); }
+bool wants_grad(const Tensor& t) {
+    if (!t.defined()) return false;
+    TORCH_CHECK(!t._fw_grad(0).defined(), "nanogpt operators have no forward-mode derivative");
+    return t.requires_grad();
+}
 
 Tensor workspace(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 
-// [..., K] as rows: their number and stride, if the rows are contiguous and do not overlap
+// [..., K] as rows: their number and stride, if they are contiguous, evenly spaced and do not overlap
 struct Rows {
     int64_t n = 0, len = 0, ld = 0;
     bool ok = false;
@@ -41,13 +47,12 @@ struct Rows {
         if (d < 1) return;
         len = t.size(d - 1);
         n = len ? t.numel() / len : 0;
-        if (t.is_contiguous()) {
-            ld = len;
-            ok = true;
-        } else if (d == 2 && (t.stride(1) == 1 || len == 1) && (t.stride(0) >= len || n <= 1)) {
-            ld = n > 1 ? t.stride(0) : len;
-            ok = true;
-        }
+        ld = len;
+        ok = t.is_contiguous() || n <= 1;
+        if (ok) return;
+        ld = d > 1 ? t.stride(d - 2) : 0;
+        ok = (t.stride(d - 1) == 1 || len == 1) && ld >= len;
+        for (int64_t i = 0; i + 2 < d; ++i) ok = ok && t.stride(i) == t.stride(i + 1) * t.size(i + 1);      // one stride for all rows
     }
 };
 
@@ -56,7 +61,7 @@ constexpr int64_t kInt = 0x7fffffff;
 // ------------------------------------------------------------------------------------------------ linear_act
 
 bool linear_usable(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& residual) {
-    if (!x.is_cuda() || !on_gpu(w, x) || !on_gpu(bias, x) || !on_gpu(residual, x)) return false;
+    if (!on_gpu(x, x) || !on_gpu(w, x) || !on_gpu(bias, x) || !on_gpu(residual, x)) return false;
     if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1)) return false;
     for (const Tensor* t : {&x, &w, &bias, &residual})
         if (t->defined() && t->scalar_type() != at::kBFloat16) return false;
@@ -97,10 +102,22 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& grad, const Ten
     return {dx, dw, db};
 }
 
-// A gradient of a gradient is not provided: say so instead of treating the gradient as a constant.
-void once(const variable_list& grads, const char* what) {
-    if (!at::GradMode::is_enabled()) return;
-    for (const Tensor& g : grads) TORCH_CHECK(!wants_grad(g), what, ": the gradient cannot be differentiated again");
+// A gradient of a gradient is not provided.  Where a graph of the backward pass is asked for, the gradients hang on what they were computed from
+// (`saved`, `grads`) by a node that raises when it is differentiated, instead of counting as constants.
+variable_list once(variable_list result, const variable_list& saved, const variable_list& grads, const char* what) {
+    if (!at::GradMode::is_enabled()) return result;
+    variable_list from{Tensor()};
+    for (const variable_list* list : {&saved, &grads})
+        for (const Tensor& t : *list)
+            if (wants_grad(t)) from.push_back(t);
+    if (from.size() == 1) return result;
+    for (Tensor& g : result)
+        if (g.defined()) {
+            from[0] = g;
+            auto refuse = std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": the gradient cannot be differentiated again", (int64_t)from.size());
+            g = (*refuse)(variable_list(from))[0];
+        }
+    return result;
 }
 
 struct LinearAct : torch::autograd::Function<LinearAct> {
@@ -112,17 +129,19 @@ struct LinearAct : torch::autograd::Function<LinearAct> {
         return out;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        once(grads, "linear_act");
         const int64_t p = ctx->saved_data["p"].toInt();
         const bool has_bias = p & 1, has_res = p & 2;
         variable_list result(5);
         if (!grads[0].defined()) return result;
         const auto saved = ctx->get_saved_variables();
+        TORCH_CHECK(linear_usable(saved[0], saved[1], Tensor(), Tensor()) && on_gpu(saved[2], saved[0]) && (!saved[2].defined() || saved[2].is_contiguous()),
+                    "linear_act: what was saved for the backward came back in another form");
         auto [dx, dw, db] = linear_backward(grads[0], saved[0], saved[1], saved[2], p >> 2, ctx->needs_input_grad(0), ctx->needs_input_grad(1),
                                             has_bias && ctx->needs_input_grad(2));
         result[0] = dx;
         result[1] = dw;
         result[2] = db;
+        result = once(std::move(result), saved, grads, "linear_act");
         if (has_res) result[3] = grads[0];
         return result;
     }
@@ -167,7 +186,7 @@ void head_strides(const Tensor& t, int64_t (&s)[3]) {
 }
 
 bool rope_call(RopeCall& c, const Tensor& q, const Tensor& k, const Tensor& cos, const Tensor& sin, const Tensor& pos, const Tensor& qw, const Tensor& kw) {
-    if (!q.is_cuda()) return false;
+    if (!on_gpu(q, q)) return false;
     for (const Tensor* t : {&k, &cos, &sin, &pos, &qw, &kw})
         if (!on_gpu(*t, q)) return false;
     const int64_t d = q.dim();
@@ -244,12 +263,11 @@ struct QKNormRope : torch::autograd::Function<QKNormRope> {
         return {qo, ko};
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        once(grads, "qk_norm_rope");
         variable_list result(9);
         if (!grads[0].defined() && !grads[1].defined()) return result;
         const auto s = ctx->get_saved_variables();
         RopeCall c;
-        TORCH_CHECK(rope_call(c, s[0], s[1], s[2], s[3], s[4], s[5], s[6]), "qk_norm_rope: unusable tensors");
+        TORCH_CHECK(rope_call(c, s[0], s[1], s[2], s[3], s[4], s[5], s[6]), "qk_norm_rope: what was saved for the backward came back in another form");
         // inputs that are tensors are numbered without the absent ones
         size_t edge = 4 + (s[4].defined() ? 1 : 0);
         const bool need_dqw = s[5].defined() && ctx->needs_input_grad(edge);
@@ -261,7 +279,7 @@ struct QKNormRope : torch::autograd::Function<QKNormRope> {
         result[1] = dk;
         result[5] = dqw;
         result[6] = dkw;
-        return result;
+        return once(std::move(result), s, grads, "qk_norm_rope");
     }
 };
 
@@ -297,7 +315,7 @@ struct DistillParams {
 };
 
 bool distill_usable(const Tensor& logits, const Tensor& ids, const Tensor& teacher, const Tensor& lse, const Tensor& weight) {
-    if (!logits.is_cuda()) return false;
+    if (!on_gpu(logits, logits)) return false;
     for (const Tensor* t : {&ids, &teacher, &lse, &weight})
         if (!on_gpu(*t, logits) || (t->defined() && !t->is_contiguous())) return false;
     if (logits.dim() != 2 || dtype_of(logits) < 0 || !Rows(logits).ok || logits.numel() == 0 || logits.size(0) > kInt || logits.size(1) > kInt) return false;
@@ -340,13 +358,14 @@ struct DistillTopK : torch::autograd::Function<DistillTopK> {
         return losses;
     }
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
-        once(grads, "distill_topk");
         variable_list result(9);
         if (!grads[0].defined()) return result;
         const auto s = ctx->get_saved_variables();
         const auto v = ctx->saved_data["p"].toDoubleVector();
+        TORCH_CHECK(distill_usable(s[0], s[1], s[2], s[3], s[4]) && on_gpu(s[5], s[0]) && s[5].is_contiguous(),
+                    "distill_topk: what was saved for the backward came back in another form");
         result[0] = distill_backward(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], {v[0], v[1], v[2], v[3]});
-        return result;
+        return once(std::move(result), s, grads, "distill_topk");
     }
 };
 

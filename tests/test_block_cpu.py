@@ -140,6 +140,10 @@ def test_fake_implementations(amd):
     assert losses.shape == (3,) and losses.dtype == torch.float32 and stats.shape == (3, 4)
     losses, grad = ops.distill_topk_fwd_bwd(m(3, 100), ids, t, None, None, 1.0, 0.0, 0.0, 0.0, 1.0)
     assert grad.shape == (3, 100) and grad.dtype == BF
+    # the functions take tensors of the meta device too
+    assert amd.linear_act(m(2, 5, 64), m(24, 64), activation="gelu").shape == (2, 5, 24)
+    assert [h.shape for h in amd.qk_norm_rope(m(9, 4, 32), m(9, 2, 32), cos, cos)] == [(9, 4, 32), (9, 2, 32)]
+    assert amd.distill_topk(m(3, 100), ids, t).shape == (3,) and amd.distill_topk_fwd_bwd(m(3, 100), ids, t)[1].shape == (3, 100)
 
 
 def test_autograd_wiring_under_fake_tensors(amd):

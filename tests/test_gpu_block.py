@@ -655,3 +655,127 @@ def test_traces_under_torch_compile(amd):
     assert torch.equal(out, eager)
     for a, e in zip(gt, ge):
         assert torch.equal(a, e)
+
+
+def three_losses(amd):
+    """(function of its leaves, the leaves) for each operator"""
+    M, K, N, V, C = 48, 64, 72, 300, 5
+    cos, sin = tables(M, 24)
+    ids, teacher, _ = teacher_rows(5, M, V, C)
+    leaves = lambda *ts: [t.requires_grad_() for t in ts]
+    yield (lambda x, w, b: (amd.linear_act(x, w, b, None, "gelu").float() * 0.5).sum()), leaves(rnd(1, M, K), rnd(2, N, K, scale=0.1), rnd(3, N))
+    yield (lambda q, k, g: sum((t.float() * 0.5).sum() for t in amd.qk_norm_rope(q, k, cos, sin, None, g))), leaves(rnd(6, M, 4, 24), rnd(7, M, 2, 24), rnd(8, 24))
+    yield (lambda l: amd.distill_topk(l, ids, teacher).sum()), leaves(rnd(9, M, V))
+
+
+def test_gradients_are_not_differentiated_again(amd):
+    """a graph of the backward pass may be asked for, but going back through it raises"""
+    for f, leaves in three_losses(amd):
+        plain = torch.autograd.grad(f(*leaves), leaves)
+        again = torch.autograd.grad(f(*leaves), leaves, create_graph=True)
+        for a, b in zip(plain, again):
+            assert torch.equal(a, b) and b.requires_grad
+            with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+                torch.autograd.grad(b.float().sum(), leaves[0], retain_graph=True)
+
+
+def test_forward_mode_is_refused(amd):
+    from torch.autograd import forward_ad
+    for f, leaves in three_losses(amd):
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward"):
+            f(forward_ad.make_dual(leaves[0].detach(), torch.ones_like(leaves[0])), *(t.detach() for t in leaves[1:]))
+
+
+def test_function_transforms_are_refused(amd):
+    for f, leaves in three_losses(amd):
+        for i in range(len(leaves)):
+            with pytest.raises(RuntimeError, match="torch.func"):
+                torch.func.grad(f, argnums=i)(*(t.detach() for t in leaves))
+
+
+def test_saved_tensors_kept_elsewhere(amd):
+    for f, leaves in three_losses(amd):
+        plain = torch.autograd.grad(f(*leaves), leaves)
+        with torch.autograd.graph.save_on_cpu():
+            loss = f(*leaves)
+        assert all(torch.equal(a, b) for a, b in zip(plain, torch.autograd.grad(loss, leaves)))
+
+
+def test_an_input_changed_before_the_backward_raises(amd):
+    for f, leaves in three_losses(amd):
+        loss = f(*leaves)
+        with torch.no_grad():
+            leaves[0].add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(loss, leaves)
+
+
+@pytest.mark.parametrize("M", [3, 40])
+def test_linear_act_views_of_a_packed_tensor(amd, M):
+    B, K, N = 3, 72, 136
+    xs, ws, rs = rnd(1, B, M, 3 * K), rnd(2, N, 2 * K, scale=0.1), rnd(3, B, M, 2 * N)
+    x, w, r = xs[..., K:2 * K], ws[:, K:], rs[..., N:]
+    assert torch.equal(amd.linear_act(x, w, None, r, "silu"), amd.linear_act(x.contiguous(), w.contiguous(), None, r.contiguous(), "silu"))
+    x2, w2 = x.transpose(0, 1), w.t().contiguous().t()        # rows that are not evenly spaced, a weight whose rows are not contiguous
+    assert torch.equal(amd.linear_act(x2, w2), amd.linear_act(x2.contiguous(), w2.contiguous()))
+
+
+def test_two_streams_at_once(amd):
+    """the same operators on two streams, different inputs, nothing between them"""
+    def inputs(seed):
+        M, K, N, V = 700, 512, 520, 4000
+        return (rnd(seed, M, K), rnd(seed + 1, N, K, scale=0.05).requires_grad_(), rnd(seed + 2, N).requires_grad_(), rnd(seed + 3, M, N),
+                rnd(seed + 4, M, V).requires_grad_(), *teacher_rows(seed + 5, M, V, 16)[:2])
+
+    def run(x, w, b, dout, logits, ids, teacher):
+        out = amd.linear_act(x, w, b, None, "silu")
+        return [out.detach(), *torch.autograd.grad(out, [w, b], dout), *amd.distill_topk_fwd_bwd(logits, ids, teacher)]
+
+    sets = [inputs(10), inputs(30)]
+    want = [[t.clone() for t in run(*s)] for s in sets]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(4):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(run(*sets[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for result in got[i]:
+            assert all(torch.equal(a, b) for a, b in zip(result, want[i]))
+
+
+def test_a_captured_training_step(amd):
+    """forward and autograd's backward in one graph; no eager graph of the leaves is alive during the capture"""
+    M, K, N, V, C = 200, 64, 96, 700, 6
+    cos, sin = tables(M, 32)
+    ids, teacher, lse = teacher_rows(10, M, V, C, 1.0)
+    ones = torch.ones(M, device="cuda")
+    leaves = {"x": rnd(1, M, K), "w": rnd(2, N, K, scale=0.1), "b": rnd(3, N), "g": 1 + rnd(4, 32, scale=0.1), "head": rnd(5, V, N, scale=0.1)}
+    leaves = {n: t.detach().requires_grad_() for n, t in leaves.items()}
+
+    def run():
+        y = amd.linear_act(leaves["x"], leaves["w"], leaves["b"], None, "silu").view(M, 3, 32)
+        h = torch.cat(amd.qk_norm_rope(y[:, :2], y[:, 2:], cos, sin, None, leaves["g"]), 1).view(M, N)
+        losses = amd.distill_topk(amd.linear_act(h, leaves["head"]), ids, teacher, lse, softcap=CAP)
+        return [losses.detach(), *torch.autograd.grad(losses, list(leaves.values()), ones)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = run()
+    for i in range(3):
+        with torch.no_grad():
+            for j, t in enumerate(leaves.values()):
+                t.mul_(1 + 0.01 * (i + 1)).add_(rnd(100 + 20 * i + j, *t.shape, scale=0.01))
+        eager = [t.clone() for t in run()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for j, (a, e) in enumerate(zip(captured, eager)):
+            assert torch.equal(a, e), (i, j)
