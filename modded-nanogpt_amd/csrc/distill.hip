@@ -663,6 +663,7 @@ int distill_args(const char* who, DistArgs& a, const void* logits, int dtype, in
     if (dtype != NGPT_DT_BF16 && dtype != NGPT_DT_F32) return fail(NGPT_EINVAL, "%s: dtype=%d", who, dtype);
     if (T <= 0 || V <= 0 || K <= 0) return fail(NGPT_EINVAL, "%s: empty problem T=%d V=%d K=%d", who, T, V, K);
     if (K > kDistMaxTop) return fail(NGPT_ERANGE, "%s: %d listed columns a row, at most %d", who, K, kDistMaxTop);
+    if (T > (1 << 30)) return fail(NGPT_ERANGE, "%s: %d rows, at most 2^30", who, T);
     if (V > (1 << 24)) return fail(NGPT_ERANGE, "%s: %d columns, at most 2^24", who, V);
     if (ld < V) return fail(NGPT_EALIGN, "%s: row stride %lld < V=%d", who, (long long)ld, V);
     if ((uintptr_t)logits % (dtype == NGPT_DT_BF16 ? 2 : 4)) return fail(NGPT_EALIGN, "%s: logits not aligned to their type", who);

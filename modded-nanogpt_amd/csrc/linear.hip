@@ -171,10 +171,12 @@ int act_grad_rows(int64_t M, int64_t N) {
     return (int)std::max<int64_t>(rows, 1);
 }
 
+constexpr int64_t kMaxStride = 1 << 21;      // values between rows: 256 rows of a tile lie within 32-bit byte offsets
+
 int check_linear(const char* who, int M, int N, int K, int act) {
     if (M <= 0 || N <= 0 || K <= 0) return fail(NGPT_EINVAL, "%s: empty problem M=%d N=%d K=%d", who, M, N, K);
     if (act < NGPT_ACT_NONE || act > NGPT_ACT_SILU) return fail(NGPT_EINVAL, "%s: activation=%d", who, act);
-    if (N > (1 << 24) || K > (1 << 24)) return fail(NGPT_ERANGE, "%s: N=%d K=%d", who, N, K);
+    if (M > (1 << 29) || N > kMaxStride || K > kMaxStride) return fail(NGPT_ERANGE, "%s: M=%d N=%d K=%d: at most 2^29 rows, 2^21 values each", who, M, N, K);
     return NGPT_OK;
 }
 
@@ -235,10 +237,9 @@ extern "C" int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* 
     if (!on16(bias_bf16)) return fail(NGPT_EALIGN, "%s: the bias starts on 16 bytes", who);
     if (ldx < K || ldw < K || (residual_bf16 && ld_residual < N))
         return fail(NGPT_EALIGN, "%s: row strides ldx=%lld ldw=%lld ld_residual=%lld", who, (long long)ldx, (long long)ldw, (long long)ld_residual);
-    // 32-bit offsets inside a tile
-    if (ldx > (1 << 21) || ldw > (1 << 21) || (residual_bf16 && ld_residual > (1 << 21)) || N > (1 << 21))
-        return fail(NGPT_ERANGE, "%s: row strides of at most 2^21 values (ldx=%lld ldw=%lld ld_residual=%lld N=%d)", who, (long long)ldx, (long long)ldw,
-                    (long long)ld_residual, N);
+    if (ldx > kMaxStride || ldw > kMaxStride || (residual_bf16 && ld_residual > kMaxStride))
+        return fail(NGPT_ERANGE, "%s: row strides of at most 2^21 values (ldx=%lld ldw=%lld ld_residual=%lld)", who, (long long)ldx, (long long)ldw,
+                    (long long)ld_residual);
     hipStream_t st = (hipStream_t)stream;
     LinearOut o{(uint16_t*)out_bf16, (uint16_t*)pre_bf16, (const uint16_t*)bias_bf16, (const uint16_t*)residual_bf16, ld_residual, M, N, 0, 0};
     o.vec = N % 8 == 0 && on16(out_bf16) && on16(pre_bf16);
@@ -269,7 +270,7 @@ struct BwdPlan {
 }  // namespace ngpt
 
 extern "C" int64_t ngpt_linear_act_bwd_workspace_bytes(int M, int N, int K) {
-    if (M <= 0 || N <= 0 || K <= 0) return 0;
+    if (M <= 0 || N <= 0 || K <= 0 || M > (1 << 29) || N > kMaxStride || K > kMaxStride) return 0;
     return BwdPlan(M, N, K).total;
 }
 
@@ -281,6 +282,8 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
         return fail(NGPT_EINVAL, "%s: null pointer", who);
     if (int e = check_linear(who, M, N, K, activation)) return e;
     if ((dw_bf16 && ldx < K) || (dx_bf16 && ldw < K)) return fail(NGPT_EALIGN, "%s: row strides ldx=%lld ldw=%lld", who, (long long)ldx, (long long)ldw);
+    if ((dw_bf16 && ldx > kMaxStride) || (dx_bf16 && ldw > kMaxStride))
+        return fail(NGPT_ERANGE, "%s: row strides of at most 2^21 values (ldx=%lld ldw=%lld)", who, (long long)ldx, (long long)ldw);
     const BwdPlan p(M, N, K);
     if (!workspace || workspace_bytes < p.total || !on16(workspace))
         return fail(NGPT_EWORKSPACE, "%s: workspace %lld < %lld bytes", who, (long long)workspace_bytes, (long long)p.total);

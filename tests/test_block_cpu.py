@@ -155,3 +155,14 @@ def test_autograd_wiring_under_fake_tensors(amd):
         loss = amd.distill_topk(torch.cat((q, k), 1).flatten(1), torch.empty(6, 2, dtype=torch.int64), torch.empty(6, 2))
         grads = torch.autograd.grad(loss.sum(), [x, w, b, r])
         assert [g.shape for g in grads] == [t.shape for t in (x, w, b, r)]
+
+
+def test_sizes_past_32_bit_offsets_are_refused(amd):
+    lib = amd._lib.load()
+    for M, N, K in (((1 << 29) + 1, 8, 64), (4, (1 << 21) + 1, 64), (4, 8, (1 << 21) + 1)):
+        assert lib.ngpt_linear_act_fwd(16, K, 16, K, None, None, 0, M, N, K, 0, 16, None, None) == -4
+        assert lib.ngpt_linear_act_bwd(16, None, 16, K, 16, K, M, N, K, 0, 16, 16, 16, 16, 1 << 60, None) == -4
+        assert lib.ngpt_linear_act_bwd_workspace_bytes(M, N, K) == 0
+    for ldx, ldw in ((1 << 22, 64), (64, 1 << 22)):
+        assert lib.ngpt_linear_act_bwd(16, None, 16, ldx, 16, ldw, 4, 8, 64, 0, 16, 16, 16, 16, 1 << 60, None) == -4
+    assert lib.ngpt_distill_fwd(16, 0, 8, 16, 0, 16, None, None, (1 << 30) + 1, 8, 2, 1.0, 0.0, 0.0, 0.0, 16, None, None) == -4

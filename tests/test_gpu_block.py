@@ -512,6 +512,64 @@ def test_distill_gradient_against_differences(amd):
         assert abs(diff - formula) < T * (h * h * 30 + 600 * E * 10 / h), (cap, diff, formula)
 
 
+# ------------------------------------------------------------------------------------------------ past 2^32 bytes
+
+def test_linear_act_of_more_than_4_gib(amd):
+    """whole numbers small enough that every sum is exact: all results are the rounded true values"""
+    M, N, K = 1_200_003, 2048, 64
+    whole = lambda seed, *shape: torch.randint(-1, 2, shape, generator=torch.Generator(D).manual_seed(seed), device=D, dtype=torch.int8).to(BF)
+    x, w, b, dout = whole(1, M, K), whole(2, N, K), whole(3, N), whole(4, M, N)
+    x, w, b = (t.requires_grad_() for t in (x, w, b))
+    out = amd.linear_act(x, w, b, None, "relu2")
+    dx, dw, db = torch.autograd.grad(out, [x, w, b], dout)
+    with torch.no_grad():
+        dw64, db64, step = torch.zeros(N, K, device=D, dtype=F64), torch.zeros(N, device=D, dtype=F64), 100_000
+        for i in range(0, M, step):
+            xs = x[i:i + step].float()
+            z = (xs @ w.float().t() + b.float()).clamp_min(0)             # at most 65
+            assert torch.equal(out[i:i + step], (z * z).to(BF)), i
+            dz = 2 * z * dout[i:i + step].float()                          # at most 130 and even: exact in bf16
+            assert torch.equal(dx[i:i + step], (dz @ w.float()).to(BF)), i
+            dw64 += dz.t() @ xs
+            db64 += dz.sum(0, dtype=F64)
+        assert torch.equal(dw, dw64.float().to(BF)) and torch.equal(db, db64.float().to(BF))
+
+
+def test_qk_norm_rope_of_more_than_4_gib(amd):
+    T, H, Dh, tail = 1_100_003, 17, 128, 1000
+    cos, sin = tables(4096, Dh)
+    pos = torch.arange(T, device=D) % 4096
+    q = torch.randn(T, H, Dh, generator=torch.Generator(D).manual_seed(1), device=D, dtype=BF).requires_grad_()
+    k = rnd(2, T // 1000 + 1, 1, Dh).repeat(1000, 1, 1)[:T].contiguous().requires_grad_()
+    qo, ko = amd.qk_norm_rope(q, k, cos, sin, pos)
+    dq, dk = torch.autograd.grad([qo, ko], [q, k], [q.detach(), k.detach()])
+    q2, k2 = (t.detach()[-tail:].clone().requires_grad_() for t in (q, k))
+    qo2, ko2 = amd.qk_norm_rope(q2, k2, cos, sin, pos[-tail:])
+    dq2, dk2 = torch.autograd.grad([qo2, ko2], [q2, k2], [q2.detach(), k2.detach()])
+    # (few tokens take another variant: two roundings of nearly the same value)
+    for a, e in ((qo, qo2), (ko, ko2), (dq, dq2), (dk, dk2)):
+        a, e = a[-tail:].detach().double(), e.detach().double()
+        assert bool(((a - e).abs() <= 2.0 ** -7 * e.abs() + 2.0 ** -18 * e.abs().max()).all())
+
+
+def test_distill_of_more_than_4_gib(amd):
+    T, V, K, tail = 44_001, 50304, 8, 64
+    ids, teacher, lse = teacher_rows(1, tail, V, K, 1.0)
+    rows = lambda t: t.repeat(T // tail + 1, *[1] * (t.ndim - 1))[-T:].contiguous()
+    logits = torch.randn(T, V, generator=torch.Generator(D).manual_seed(2), device=D, dtype=BF)
+    ids, teacher, lse = rows(ids), rows(teacher), rows(lse)
+    losses, grad = amd.distill_topk_fwd_bwd(logits, ids, teacher, lse, softcap=CAP)
+    few = amd.distill_topk_fwd_bwd(logits[-tail:], ids[-tail:], teacher[-tail:], lse[-tail:], softcap=CAP)
+    assert torch.equal(losses[-tail:], few[0]) and torch.equal(grad[-tail:], few[1])
+    del grad
+    leaf = logits.requires_grad_()
+    (g,) = torch.autograd.grad(amd.distill_topk(leaf, ids, teacher, lse, softcap=CAP), [leaf], torch.ones(T, device=D))
+    last = logits.detach()[-tail:].clone().requires_grad_()
+    (g2,) = torch.autograd.grad(amd.distill_topk(last, ids[-tail:], teacher[-tail:], lse[-tail:], softcap=CAP), [last], torch.ones(tail, device=D))
+    # (few rows take another sweep width: the sums' order differs; a gradient's terms are off by some 2^-20 and the store by 2^-8)
+    assert float((g[-tail:].double() - g2.double()).abs().max()) <= 2.0 ** -7 * float(g2.double().abs().max())
+
+
 # ------------------------------------------------------------------------------------------------ together
 
 def step(fn_linear, fn_rope, fn_loss, p, B, T, H, Hk, Dh):
