@@ -91,6 +91,7 @@ __global__ __launch_bounds__(256) void transpose_pad_kernel(const uint16_t* __re
 
 // dz = dout act'(z) (zeros in the padding of its [rows_p, cols_p]) and the column sums of dz, in fp32 before dz is rounded: a workgroup
 // covers 256 columns and every gridDim.y-th group of 8 rows, its sums go to part[blockIdx.y][N].  dz or part may be null.
+// 16384 x 4096 with gelu_tanh: 70 to 72 us (403 MB, 5.6 TB/s, partly from the cache); sums alone, 49152 x 768: 13 us.
 constexpr int kColsPerBlock = 256, kRowLanes = 8;
 template <int ACT>
 __global__ __launch_bounds__(256) void act_grad_kernel(const uint16_t* __restrict__ dout, const uint16_t* __restrict__ pre, int M, int N,

@@ -12,6 +12,10 @@
 // Layout of the work: a row belongs to LPR lanes of 8 consecutive values each (D <= 8 LPR), a wave holds 64 / LPR rows,
 // which are consecutive heads of ONE token: their loads are one contiguous piece and they share the cos / sin values,
 // which stay in registers while the wave walks the token's heads.  U steps of loads are issued before the first is used.
+//
+// Measured: 49152 tokens x 12 bf16 heads of 128, 64 values turned: forward 58 us (302 MB, 5.2 TB/s), backward 97 us (453 MB, 4.7 TB/s); a large
+// copy reaches 5.1 on this card.  8193 tokens x 16 fp32 heads of 80 with weights: 22 and 28 us, their sums 4 us.  16 tokens x 20 heads: 4.6 us,
+// of which an empty launch is about 2.5 and the rest two dependent round trips (the position, then its row of the tables).
 #include "common.h"
 #include "host_util.h"
 #include <algorithm>

@@ -1,7 +1,7 @@
 // Host side of linear_act, qk_norm_rope and distill_topk for torch: checks that the tensors can be used as they are, allocates results and
 // workspaces, calls the C ABI on the tensors' GPU and its current stream, and records the gradient functions.  Python adds the argument
 // messages, the copies of tensors that cannot be used as they are, and the registered operators.  (Written in C++ because a call costs
-// 4 us of host time this way and 12 to 20 from Python, more than the kernels take for one token; gradients run without the interpreter.)
+// 5 to 8 us of host time this way and 12 to 17 from Python, more than the kernels take for one token; gradients run without the interpreter.)
 //
 // Functions that may be given anything return None for tensors they cannot use as they are; the *_raw ones raise.
 #include <ATen/ATen.h>
