@@ -12,25 +12,25 @@ namespace ngpt {
 __device__ __forceinline__ float normal_cdf(float z, float& gauss) {
     gauss = __builtin_amdgcn_exp2f(-0.5f * 1.4426950408889634f * z * z);
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(fabsf(z), 0.3275911f * 0.70710678118654752f, 1.0f));
-    float p = __builtin_fmaf(t, 1.061405429f, -1.453152027f);
-    p = __builtin_fmaf(t, p, 1.421413741f);
-    p = __builtin_fmaf(t, p, -0.284496736f);
-    p = __builtin_fmaf(t, p, 0.254829592f);
-    const float tail = 0.5f * p * t * gauss;
+    float p = __builtin_fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+    p = __builtin_fmaf(t, p, 0.5f * 1.421413741f);
+    p = __builtin_fmaf(t, p, 0.5f * -0.284496736f);
+    p = __builtin_fmaf(t, p, 0.5f * 0.254829592f);
+    const float tail = p * t * gauss;
     return z < 0.0f ? tail : 1.0f - tail;
 }
 template <int ACT>
 __device__ __forceinline__ float act_of(float z) {
     constexpr float kLog2e = 1.4426950408889634f;
     if constexpr (ACT == NGPT_ACT_RELU2) {
-        const float r = fmaxf(z, 0.0f);
-        return z != z ? z : r * r;
+        const float r = __builtin_elementwise_maximum(z, 0.0f);      // (keeps a NaN, in one instruction)
+        return r * r;
     } else if constexpr (ACT == NGPT_ACT_GELU) {
         float gauss;
         return z * normal_cdf(z, gauss);
     } else if constexpr (ACT == NGPT_ACT_GELU_TANH) {      // z (1 + tanh u) / 2 = z sigmoid(2 u)
-        const float u = z * __builtin_fmaf(z * z, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
-        return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.0f * kLog2e * u));
+        constexpr float c = -2.0f * kLog2e * 0.7978845608028654f;
+        return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * __builtin_fmaf(z * z, c * 0.044715f, c)));
     } else if constexpr (ACT == NGPT_ACT_SILU) {
         return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
     } else {
@@ -41,7 +41,7 @@ template <int ACT>
 __device__ __forceinline__ float act_slope(float z) {
     constexpr float kLog2e = 1.4426950408889634f;
     if constexpr (ACT == NGPT_ACT_RELU2) {
-        return z != z ? z : 2.0f * fmaxf(z, 0.0f);
+        return 2.0f * __builtin_elementwise_maximum(z, 0.0f);
     } else if constexpr (ACT == NGPT_ACT_GELU) {
         float gauss;
         const float cdf = normal_cdf(z, gauss);
