@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import torch
 from torch import Tensor
+from torch.compiler import is_dynamo_compiling
 
 from . import _lib
 
@@ -161,12 +162,13 @@ def linear_act(x: Tensor, w: Tensor, bias: Tensor | None = None, residual: Tenso
     and residual applied to the fp32 sums, one rounding.  `activation`: "none", "relu2" (max(z, 0)^2), "gelu", "gelu_tanh", "silu".
     Any sizes; rows of x, w and residual may be strided.  Differentiable in x, w, bias and residual; an activation's backward keeps
     the bf16 pre-activation."""
-    if _plain(x, w, bias, residual):
+    if not is_dynamo_compiling():       # straight to the binding, which takes ordinary tensors in usable form
         act = ACTIVATIONS.get(activation)
         if act is not None:
-            out = _b().linear_act(x, w, bias, residual, act)
+            out = (_binding or _b()).linear_act(x, w, bias, residual, act)
             if out is not None:
                 return out
+    if _plain(x, w, bias, residual):
         act = _linear_shapes(x, w, bias, residual, activation)
         if _direct(x, w, bias, residual):
             _same_gpu(x, w, bias, residual)
@@ -263,10 +265,11 @@ def qk_norm_rope(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor, positions: Tens
     sequence).  A position outside the tables makes that token's heads NaN.  2 <= D <= 512.  Differentiable in q, k and the weights."""
     eps = RMS_EPS if eps is None else float(eps)
     tensors = (q, k, cos, sin, positions, q_weight, k_weight)
-    if _plain(*tensors):
-        out = _b().qk_norm_rope(*tensors, eps, interleaved)
+    if not is_dynamo_compiling():
+        out = (_binding or _b()).qk_norm_rope(*tensors, eps, interleaved)
         if out is not None:
             return out
+    if _plain(*tensors):
         _rope_shapes(*tensors)
         if _direct(*tensors):
             _same_gpu(*tensors)
@@ -388,10 +391,11 @@ def distill_topk(logits: Tensor, ids: Tensor, teacher: Tensor, teacher_lse: Tens
     Differentiable in logits only."""
     tensors = (logits, ids, teacher, teacher_lse, row_weight)
     params = (float(temperature), *_softcap(softcap))
-    if _plain(*tensors):
-        losses = _b().distill_topk(*tensors, *params)
+    if not is_dynamo_compiling():
+        losses = (_binding or _b()).distill_topk(*tensors, *params)
         if losses is not None:
             return losses
+    if _plain(*tensors):
         _distill_shapes(*tensors)
         if _direct(*tensors):
             _same_gpu(*tensors)
@@ -407,10 +411,11 @@ def distill_topk_fwd_bwd(logits: Tensor, ids: Tensor, teacher: Tensor, teacher_l
     row fits a workgroup's registers (53744 columns), two beyond.  Not differentiable itself."""
     tensors = (logits, ids, teacher, teacher_lse, row_weight)
     params = (float(temperature), *_softcap(softcap), float(grad_scale))
-    if _plain(*tensors):
-        out = _b().distill_fused(*tensors, *params)
+    if not is_dynamo_compiling():
+        out = (_binding or _b()).distill_fused(*tensors, *params)
         if out is not None:
             return out
+    if _plain(*tensors):
         _distill_shapes(*tensors)
         if _direct(*tensors):
             _same_gpu(*tensors)

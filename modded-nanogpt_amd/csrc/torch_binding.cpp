@@ -1,14 +1,17 @@
 // Host side of linear_act, qk_norm_rope and distill_topk for torch: checks that the tensors can be used as they are, allocates results and
 // workspaces, calls the C ABI on the tensors' GPU and its current stream, and records the gradient functions.  Python adds the argument
 // messages, the copies of tensors that cannot be used as they are, and the registered operators.  (Written in C++ because a call costs
-// 5 to 8 us of host time this way and 12 to 17 from Python, more than the kernels take for one token; gradients run without the interpreter.)
+// 4 to 5 us of host time this way and 12 to 17 from Python, more than the kernels take for one token; gradients run without the interpreter.)
 //
 // Functions that may be given anything return None for tensors they cannot use as they are; the *_raw ones raise.
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/object_ptr.h>
 #include <torch/csrc/utils/pybind.h>
 #include "../../include/ngpt_fp8.h"
 
@@ -407,16 +410,107 @@ Pair distill_fused(const Tensor& logits, const Tensor& ids, const Tensor& teache
     return std::make_tuple(losses, grad);
 }
 
+// ------------------------------------------------------------------------------------------------ for Python
+
+// The public functions' first call, without pybind's conversions (they take 1 us): positional arguments only.  None is returned for anything but
+// ordinary tensors in usable form.
+struct Given {
+    PyObject* const* args;
+    bool ok = true;
+
+    OptTensor maybe(int i) {
+        PyObject* o = args[i];
+        if (o == Py_None) return std::nullopt;
+        if (!THPVariable_CheckTypeExact(Py_TYPE(o))) {      // Tensor or Parameter: a subclass may mean something else
+            ok = false;
+            return std::nullopt;
+        }
+        return THPVariable_Unpack(o);
+    }
+    Tensor tensor(int i) {
+        OptTensor t = maybe(i);
+        ok = ok && t.has_value();
+        return t.has_value() ? std::move(*t) : Tensor();
+    }
+    double number(int i) {
+        const double v = PyFloat_AsDouble(args[i]);
+        if (v == -1.0 && PyErr_Occurred()) throw python_error();
+        return v;
+    }
+    int64_t integer(int i) {
+        const int64_t v = PyLong_AsLongLong(args[i]);
+        if (v == -1 && PyErr_Occurred()) throw python_error();
+        return v;
+    }
+};
+
+PyObject* to_python(OptTensor t) {
+    if (!t.has_value()) Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(*t));
+}
+PyObject* to_python(Pair t) {
+    if (!t.has_value()) Py_RETURN_NONE;
+    THPObjectPtr a(THPVariable_Wrap(std::move(std::get<0>(*t)))), b(THPVariable_Wrap(std::move(std::get<1>(*t))));
+    return a && b ? PyTuple_Pack(2, a.get(), b.get()) : nullptr;
+}
+
+PyObject* py_linear_act(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 5, "linear_act: 5 arguments");
+    Given g{args};
+    const Tensor x = g.tensor(0), w = g.tensor(1);
+    const OptTensor bias = g.maybe(2), residual = g.maybe(3);
+    if (!g.ok) Py_RETURN_NONE;
+    return to_python(linear_act(x, w, bias, residual, g.integer(4)));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 9, "qk_norm_rope: 9 arguments");
+    Given g{args};
+    const Tensor q = g.tensor(0), k = g.tensor(1), cos = g.tensor(2), sin = g.tensor(3);
+    const OptTensor pos = g.maybe(4), qw = g.maybe(5), kw = g.maybe(6);
+    if (!g.ok) Py_RETURN_NONE;
+    return to_python(qk_norm_rope(q, k, cos, sin, pos, qw, kw, g.number(7), g.integer(8) != 0));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_distill_topk(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 9, "distill_topk: 9 arguments");
+    Given g{args};
+    const Tensor logits = g.tensor(0), ids = g.tensor(1), teacher = g.tensor(2);
+    const OptTensor lse = g.maybe(3), weight = g.maybe(4);
+    if (!g.ok) Py_RETURN_NONE;
+    return to_python(distill_topk(logits, ids, teacher, lse, weight, g.number(5), g.number(6), g.number(7), g.number(8)));
+    END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_distill_fused(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    TORCH_CHECK(n == 10, "distill_fused: 10 arguments");
+    Given g{args};
+    const Tensor logits = g.tensor(0), ids = g.tensor(1), teacher = g.tensor(2);
+    const OptTensor lse = g.maybe(3), weight = g.maybe(4);
+    if (!g.ok) Py_RETURN_NONE;
+    return to_python(distill_fused(logits, ids, teacher, lse, weight, g.number(5), g.number(6), g.number(7), g.number(8), g.number(9)));
+    END_HANDLE_TH_ERRORS
+}
+
+template <PyObject* (*F)(PyObject*, PyObject* const*, Py_ssize_t)>
+PyMethodDef method(const char* name) { return {name, (PyCFunction)(void (*)(void))F, METH_FASTCALL, nullptr}; }
+
+PyMethodDef methods[] = {method<py_linear_act>("linear_act"), method<py_qk_norm_rope>("qk_norm_rope"), method<py_distill_topk>("distill_topk"),
+                         method<py_distill_fused>("distill_fused"), {nullptr, nullptr, 0, nullptr}};
+
 }  // namespace
 
 PYBIND11_MODULE(_ngpt_torch, m) {
-    m.def("linear_act", &linear_act);
+    if (PyModule_AddFunctions(m.ptr(), methods) != 0) throw pybind11::error_already_set();
     m.def("linear_raw", &linear_raw);
     m.def("linear_backward_raw", &linear_backward_raw);
-    m.def("qk_norm_rope", &qk_norm_rope);
     m.def("rope_backward_raw", &rope_backward_raw);
-    m.def("distill_topk", &distill_topk);
     m.def("distill_raw", &distill_raw);
     m.def("distill_backward_raw", &distill_backward_raw);
-    m.def("distill_fused", &distill_fused);
 }
