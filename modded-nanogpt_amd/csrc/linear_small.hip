@@ -203,9 +203,12 @@ __global__ __launch_bounds__(256 * KG, KG == 4 ? 4 : 2) void linear_mid_kernel(L
         if ((kt0 + kt) * 64 + 64 <= K) {
 #pragma unroll
             for (int i = 0; i < Cfg::LOADS; ++i) __builtin_memcpy(&reg[i], (i < Cfg::LOADS / 2 ? wt : xt) + off[i] + k, 16);
+        } else if (K >= 8) {
+#pragma unroll
+            for (int i = 0; i < Cfg::LOADS; ++i) reg[i] = load_row8_end((i < Cfg::LOADS / 2 ? wt : xt) + off[i], k, K);
         } else {
 #pragma unroll
-            for (int i = 0; i < Cfg::LOADS; ++i) reg[i] = load_row8((i < Cfg::LOADS / 2 ? wt : xt) + off[i], k, K);
+            for (int i = 0; i < Cfg::LOADS; ++i) reg[i] = load_row8_short((i < Cfg::LOADS / 2 ? wt : xt) + off[i], k, K);
         }
     };
     auto put = [&](int stage, const v4i (&reg)[Cfg::LOADS]) {
