@@ -178,9 +178,10 @@ __device__ __forceinline__ void linear_epilogue(const LinearOut& o, v16f (&acc)[
     };
     // a block between memory and the staging area where rows start anywhere: 16 bytes at any byte address, the row's last values one by one
     auto block_slow = [&](int tn, const uint16_t* from, uint16_t* to, int64_t ld) {
+        const int left = N - f;
 #pragma unroll 1
         for (int k = 0; k < NI; ++k) {
-            const int row = RPI * k + rd_row, m = m0 + tn * 32 + row, left = N - f;
+            const int row = RPI * k + rd_row, m = m0 + tn * 32 + row;
             uint8_t* at = stage + swz(row, rd_chunk);
             if (m < o.M && left > 0) {
                 if (to) store_any(to + (int64_t)m * ld + f, *(const v4i*)at, left);
@@ -188,6 +189,8 @@ __device__ __forceinline__ void linear_epilogue(const LinearOut& o, v16f (&acc)[
             }
         }
     };
+    // All pieces at once where the block's rows and the lane's 8 values all exist (not in the large tiles' kernel: see the number of blocks above)
+    auto whole_block = [&](int tn) { return TN <= 2 && m0 + tn * 32 + 32 <= o.M && f + 8 <= N; };
     auto store_block = [&](int tn, __amdgpu_buffer_rsrc_t buf, uint16_t* to) {
         if (o.vec) {
 #pragma unroll
@@ -196,6 +199,13 @@ __device__ __forceinline__ void linear_epilogue(const LinearOut& o, v16f (&acc)[
                 const v4i v = *(const v4i*)(stage + swz(row, rd_chunk));
                 __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), buf, in ? off + (tn * 32 + RPI * k) * N * 2 : kNowhere, 0, 2);
             }
+        } else if (whole_block(tn)) {
+            uint16_t* const at = to + (int64_t)(m0 + tn * 32 + rd_row) * N + f;
+            v4i v[NI];
+#pragma unroll
+            for (int k = 0; k < NI; ++k) v[k] = *(const v4i*)(stage + swz(RPI * k + rd_row, rd_chunk));
+#pragma unroll
+            for (int k = 0; k < NI; ++k) __builtin_memcpy(at + (int64_t)(RPI * k) * N, &v[k], 16);
         } else {
             block_slow(tn, nullptr, to, N);
         }
@@ -228,6 +238,13 @@ __device__ __forceinline__ void linear_epilogue(const LinearOut& o, v16f (&acc)[
 #pragma unroll
                 for (int k = 0; k < NI; ++k) *(v4i*)(stage + swz(RPI * k + rd_row, rd_chunk)) = line[k];
                 if (tn + 1 < TN) load_block(tn + 1);       // in flight while this block is worked on
+            } else if (whole_block(tn)) {
+                const uint16_t* const at = o.res + (int64_t)(m0 + tn * 32 + rd_row) * o.ld_res + f;
+                v4i v[NI];
+#pragma unroll
+                for (int k = 0; k < NI; ++k) __builtin_memcpy(&v[k], at + (int64_t)(RPI * k) * o.ld_res, 16);
+#pragma unroll
+                for (int k = 0; k < NI; ++k) *(v4i*)(stage + swz(RPI * k + rd_row, rd_chunk)) = v[k];
             } else {
                 block_slow(tn, o.res, nullptr, o.ld_res);
             }
