@@ -60,7 +60,8 @@ int ngpt_num_cus(void);
  * No counterpart in the reference (contributors patch torch.profiler in by hand).  When enabled,
  * the heavy launches of the fused lm_head + CE path are bracketed by HIP events on their own
  * stream.  Slots: 0 fused CE forward kernel, 1 dlogits recompute, 2 dx GEMM, 3 dW GEMM (of the fused CE backward),
- * 4 other fp8 GEMMs, 5 up projection + ReLU^2, 6 dpre, 7 plain bf16 GEMMs of the MLP, 8 MLP input producers.
+ * 4 other fp8 GEMMs, 5 up projection + ReLU^2, 6 dpre, 7 plain bf16 GEMMs of the MLP and of linear_act,
+ * 8 MLP input producers and qk_norm_rope.
  * ngpt_profile_read waits for the recorded launches of a slot, returns the sum of their
  * durations and their count, and clears the slot. */
 int ngpt_profile_enable(int on);
@@ -342,7 +343,7 @@ int ngpt_lmhead_ce_bwd_codes(const void* x_f8, const void* w_f8_vk, const int64_
  * out [M, N] = residual + act(x [M, K] . w [N, K]^T + bias [N]), bf16 in and out, fp32 in between, rounded once.  bias and residual are nullable.
  * The bias starts on 16 bytes.
  * Row strides in elements, at most 2^21; rows may start anywhere (the fastest kernel for many rows needs K % 64 == 0 and rows of x and w on 16 bytes).
- * Any M, N, K.  pre [M, N] (nullable; null for NGPT_ACT_NONE) receives bf16(x w^T + bias), what the backward of an
+ * M up to 2^29, N and K up to 2^21.  pre [M, N] (nullable; null for NGPT_ACT_NONE) receives bf16(x w^T + bias), what the backward of an
  * activation needs. */
 int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw, const void* bias_bf16,
                         const void* residual_bf16, int64_t ld_residual, int M, int N, int K, int activation,
@@ -360,8 +361,8 @@ int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, const void*
  * y = rot(x * rsqrt(mean(x^2) + eps) * weight) for every head of q [B, T, Hq, D] and k [B, T, Hk, D] (`dtype`), one pass over both.
  * The first R of a head's D values are rotated as R / 2 pairs (a, b) -> (a cos - b sin, b cos + a sin): pairs (i, i + R / 2), or
  * (2 i, 2 i + 1) with `interleaved`.  cos_tab / sin_tab [P, R / 2] (`tab_dtype`), a row per position; `positions` [B, T] int32 or
- * int64 (nullable: the token's index in its sequence, T <= P).  A position outside 0 .. P - 1 makes the token's heads NaN and reads
- * nothing.  Strides are host arrays in elements: {batch, token, head} for q and k, {batch, token} for positions; the D values of a head are
+ * int64 (nullable: the token's index in its sequence, T <= P).  A position outside 0 .. P - 1 makes the token's heads NaN; nothing
+ * outside the tables is read.  Strides are host arrays in elements: {batch, token, head} for q and k, {batch, token} for positions; the D values of a head are
  * contiguous.  Weights [D] in `dtype`, nullable.  Outputs are contiguous [B, T, H, D].  2 <= D <= 512, R even, 2 <= R <= D. */
 int ngpt_qk_norm_rope(const void* q, const int64_t* q_strides, const void* k, const int64_t* k_strides, int dtype,
                       int B, int T, int Hq, int Hk, int D, int R, const void* cos_tab, const void* sin_tab, int tab_dtype, int P,
@@ -381,7 +382,8 @@ int ngpt_qk_norm_rope_bwd(const void* dq_out, const int64_t* dq_strides, const v
                           void* workspace, int64_t workspace_bytes, void* stream);
 
 /* ---- distillation from a teacher's top logits --------------------------------------------------
- * Row by row, z = softcap(logits) / temperature, softcap(l) = A sigmoid((l + B) / C) (C == 0: no softcap), q = softmax(z) over V columns.
+ * Row by row, z = softcap(logits) / temperature, softcap(l) = A sigmoid((l + B) / C) (C == 0: no softcap), q = softmax(z) over V columns;
+ * A / temperature <= 80.
  * ids [T, K] (int32 or int64) and teacher [T, K] fp32 list a teacher's logits of K columns.  p = softmax of the listed teacher / temperature;
  * or, with teacher_lse [T] (the teacher's log-sum-exp over all of ITS columns at this temperature), p = exp(teacher / temperature - lse),
  * and the rest of the teacher's mass stands against the rest of the student's:

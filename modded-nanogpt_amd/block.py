@@ -160,7 +160,7 @@ linear_act_op.register_autograd(_linear_backward, setup_context=_linear_setup)
 def linear_act(x: Tensor, w: Tensor, bias: Tensor | None = None, residual: Tensor | None = None, activation: str = "none") -> Tensor:
     """residual + act(x @ w.T + bias) for bf16 x [..., K], w [N, K], bias [N], residual [..., N]; fp32 accumulation, bias, activation
     and residual applied to the fp32 sums, one rounding.  `activation`: "none", "relu2" (max(z, 0)^2), "gelu", "gelu_tanh", "silu".
-    Any sizes; rows of x, w and residual may be strided.  Differentiable in x, w, bias and residual; an activation's backward keeps
+    Any sizes (2^29 rows, 2^21 values in one); rows of x, w and residual may be strided.  Differentiable in x, w, bias and residual; an activation's backward keeps
     the bf16 pre-activation."""
     if not is_dynamo_compiling():       # straight to the binding, which takes ordinary tensors in usable form
         act = ACTIVATIONS.get(activation)
@@ -380,7 +380,7 @@ def _softcap(softcap) -> tuple[float, float, float]:
 def distill_topk(logits: Tensor, ids: Tensor, teacher: Tensor, teacher_lse: Tensor | None = None, row_weight: Tensor | None = None,
                  temperature: float = 1.0, softcap: tuple[float, float, float] | None = None) -> Tensor:
     """losses [T] fp32 of the student's logits [T, V] (bf16 or fp32) against a teacher's logits `teacher` [T, K] fp32 of the columns `ids`
-    [T, K] (int32 or int64), K <= 512.  With z = softcap(logits) / temperature, softcap(l) = A sigmoid((l + B) / C) for
+    [T, K] (int32 or int64), K <= 512, V <= 2^24, A / temperature <= 80.  With z = softcap(logits) / temperature, softcap(l) = A sigmoid((l + B) / C) for
     softcap = (A, B, C), and q = softmax(z) over all V columns,
 
         losses = row_weight temperature^2 sum_j p_j (log p_j - log q[ids_j]),    p = softmax(teacher / temperature) over the list,

@@ -65,8 +65,8 @@ enum ProfileSlot : int {
     PROF_GEMM = 4,        // any other fp8 GEMM launch (nanogpt::mm forward / backward, the FP8 down projection)
     PROF_FC_RELU2 = 5,    // up projection with the ReLU^2 epilogue (fp8 or bf16 operands)
     PROF_DPRE = 6,        // dpre GEMM of the MLP backward
-    PROF_GEMM_BF16 = 7,   // plain bf16 GEMMs of the MLP (c_proj, dx, dW1, dW2), their summing pass included
-    PROF_PRODUCERS = 8,   // rms-norm + amax + quantise of the MLP input, the norm's backward
+    PROF_GEMM_BF16 = 7,   // plain bf16 GEMMs of the MLP (c_proj, dx, dW1, dW2) and of linear_act, their summing pass included
+    PROF_PRODUCERS = 8,   // rms-norm + amax + quantise of the MLP input, the norm's backward, qk_norm_rope
     PROF_SLOTS = 9
 };
 bool profiling_on();

@@ -316,6 +316,7 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
         if (int e = transpose_pad((const uint16_t*)w_bf16, ldw, N, K, wt, (int)p.N64, st)) return e;
         LinearOut o{(uint16_t*)dx_bf16, nullptr, nullptr, nullptr, 0, M, K, K % 8 == 0 && on16(dx_bf16), 0};
         // (dz's padding and w^T's are zeros)
+        ProfileScope prof(PROF_GEMM_BF16, st);
         if (int e = linear_run(o, dz, ld_dz, wt, p.N64, own_dz ? (int)p.N64 : N, NGPT_ACT_NONE, st)) return e;
     }
     if (dw_bf16) {      // dw [N, K] = dz^T . x, contraction over the M rows of both
