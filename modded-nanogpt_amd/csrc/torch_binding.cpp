@@ -5,7 +5,9 @@
 //
 // Functions that may be given anything return None for tensors they cannot use as they are; the *_raw ones raise.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -413,10 +415,10 @@ Pair distill_fused(const Tensor& logits, const Tensor& ids, const Tensor& teache
 // ------------------------------------------------------------------------------------------------ for Python
 
 // The public functions' first call, without pybind's conversions (they take 1 us): positional arguments only.  None is returned for anything but
-// ordinary tensors in usable form.
+// ordinary tensors in usable form, and under a dispatch mode (a tracer, a counter of operations), which has to see the registered operator.
 struct Given {
     PyObject* const* args;
-    bool ok = true;
+    bool ok = !c10::impl::TorchDispatchModeTLS::any_modes_set() && !at::tracer::impl::is_dispatch_enabled();
 
     OptTensor maybe(int i) {
         PyObject* o = args[i];

@@ -837,3 +837,40 @@ def test_a_captured_training_step(amd):
         torch.cuda.synchronize()
         for j, (a, e) in enumerate(zip(captured, eager)):
             assert torch.equal(a, e), (i, j)
+
+
+def test_dispatch_modes_see_the_registered_operators(amd):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Names(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            seen.append(func.__name__ if hasattr(func, "__name__") else str(func))
+            return func(*args, **(kwargs or {}))
+
+    names = ("linear_act", "qk_norm_rope", "distill_topk")
+    for name, (f, leaves) in zip(names, three_losses(amd)):
+        plain = torch.autograd.grad(f(*leaves), leaves)
+        seen = []
+        with Names():
+            grads = torch.autograd.grad(f(*leaves), leaves)
+        assert any(n.startswith(name + ".") for n in seen) and any(n.startswith(name + "_backward") for n in seen), seen
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+    ids, teacher, _ = teacher_rows(5, 4, 300, 5)
+    seen = []
+    logits = rnd(1, 4, 300)
+    with Names():
+        a = amd.distill_topk_fwd_bwd(logits, ids, teacher)
+    assert any(n.startswith("distill_topk_fwd_bwd") for n in seen)
+    assert all(torch.equal(x, y) for x, y in zip(a, amd.distill_topk_fwd_bwd(logits, ids, teacher)))
+
+
+def test_a_traced_function_holds_the_registered_operator(amd):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x, w = rnd(1, 5, 64), rnd(2, 24, 64)
+    g = make_fx(lambda x, w: amd.linear_act(x, w, activation="silu"))(x, w)
+    assert "nanogpt.linear_act" in g.code
+    y = rnd(3, 5, 64)
+    assert torch.equal(g(y, w), amd.linear_act(y, w, activation="silu"))
+    h = torch.jit.trace(lambda x, w: amd.linear_act(x, w, activation="silu"), (x, w))
+    assert "nanogpt::linear_act" in str(h.graph)
+    assert torch.equal(h(y, w), amd.linear_act(y, w, activation="silu"))
