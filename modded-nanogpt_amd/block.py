@@ -50,12 +50,7 @@ def _plain(*tensors: Tensor | None) -> bool:
 
 def _rows(t: Tensor | None) -> Tensor | None:
     """[..., K] whose rows are contiguous, evenly spaced and do not overlap: itself, or a copy."""
-    if t is None or t.is_contiguous() or t.ndim == 0:
-        return t
-    if (t.ndim > 1 and (t.stride(-1) == 1 or t.shape[-1] == 1) and t.stride(-2) >= t.shape[-1]
-            and all(t.stride(i) == t.stride(i + 1) * t.shape[i + 1] for i in range(t.ndim - 2))):
-        return t
-    return t.contiguous()
+    return t if t is None or t.ndim == 0 or _b().rows_in_place(t) else t.contiguous()
 
 
 def _direct(*tensors: Tensor | None) -> bool:

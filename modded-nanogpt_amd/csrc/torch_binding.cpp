@@ -43,7 +43,8 @@ bool wants_grad(const Tensor& t) {
 
 Tensor workspace(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 
-// [..., K] as rows: their number and stride, if they are contiguous, evenly spaced and do not overlap
+// [..., K] as rows: their number and stride, if each is contiguous and they are evenly spaced and do not overlap.  A dimension of size one has no
+// stride that counts, but the values of a single row have: a column of a matrix is one row, `size` apart.
 struct Rows {
     int64_t n = 0, len = 0, ld = 0;
     bool ok = false;
@@ -53,10 +54,12 @@ struct Rows {
         len = t.size(d - 1);
         n = len ? t.numel() / len : 0;
         ld = len;
-        ok = t.is_contiguous() || n <= 1;
+        ok = t.is_contiguous();
+        if (ok || (len > 1 && t.stride(d - 1) != 1)) return;
+        ok = n <= 1;
         if (ok) return;
         ld = d > 1 ? t.stride(d - 2) : 0;
-        ok = (t.stride(d - 1) == 1 || len == 1) && ld >= len;
+        ok = ld >= len;
         for (int64_t i = 0; i + 2 < d; ++i) ok = ok && t.stride(i) == t.stride(i + 1) * t.size(i + 1);      // one stride for all rows
     }
 };
@@ -510,6 +513,7 @@ PyMethodDef methods[] = {method<py_linear_act>("linear_act"), method<py_qk_norm_
 
 PYBIND11_MODULE(_ngpt_torch, m) {
     if (PyModule_AddFunctions(m.ptr(), methods) != 0) throw pybind11::error_already_set();
+    m.def("rows_in_place", [](const Tensor& t) { return Rows(t).ok; });      // the one rule for Python's copies too; looks at sizes and strides only
     m.def("linear_raw", &linear_raw);
     m.def("linear_backward_raw", &linear_backward_raw);
     m.def("rope_backward_raw", &rope_backward_raw);

@@ -1,0 +1,54 @@
+"""Which layouts the block operators read in place: the binding's rule on CPU tensors, whose sizes and strides alone it looks at."""
+import itertools
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def rows_in_place():
+    import modded_nanogpt_amd
+    if not modded_nanogpt_amd._lib.BINDING_PATH.exists():
+        from modded_nanogpt_amd.build import build
+        build(verbose=False)
+    return modded_nanogpt_amd._lib.load_torch().rows_in_place
+
+
+def offsets(t):
+    """where each value of t lies in its storage, as [rows, values of a row]"""
+    at = torch.zeros(t.shape, dtype=torch.int64)
+    for d in range(t.ndim):
+        shape = [1] * t.ndim
+        shape[d] = t.shape[d]
+        at = at + (torch.arange(t.shape[d]) * t.stride(d)).view(shape)
+    return at.reshape(-1, t.shape[-1]) if t.shape[-1] else at.reshape(0, 0)
+
+
+def readable(t):
+    """one start, one distance: row r is at r * distance, value by value, and no two rows overlap"""
+    at = offsets(t)
+    if at.numel() == 0:
+        return True
+    n, length = at.shape
+    apart = int(at[1, 0]) if n > 1 else length
+    return apart >= length and bool((at == torch.arange(n)[:, None] * apart + torch.arange(length)).all())
+
+
+def test_a_single_row_of_another_stride_is_not_read_in_place(rows_in_place):
+    m = torch.zeros(64, 48)
+    for t in (m[:, 3], m.t()[3], m.t()[:1], m[:1, ::2], m[0, ::2], torch.zeros(1, 48, 5)[:, :, -1], torch.zeros(1, 48, 5).transpose(1, 2)[:, -1],
+              torch.zeros(1).expand(48), torch.zeros(1, 1).expand(1, 48), torch.zeros(1, 1, 1).expand(1, 1, 48)):
+        assert not readable(t) and not rows_in_place(t), (t.shape, t.stride())
+    for t in (m[5], m[5:6], m[5:6, 7:20], m[5, 7:20], m[:1, :1], m[:, :1][3], torch.zeros(1, 5, 48)[:, -1], m[:, 3][:1], torch.zeros(1, 1).expand(1, 1)):
+        assert readable(t) and rows_in_place(t), (t.shape, t.stride())
+
+
+def test_what_is_read_in_place_is_where_the_kernels_look(rows_in_place):
+    base, taken = torch.zeros(4 * 5 * 6 * 7), 0
+    for shape in ((7,), (1,), (0,), (3, 4), (1, 4), (4, 1), (1, 1), (3, 0), (0, 3), (2, 3, 4), (1, 3, 4), (2, 1, 4), (2, 3, 1), (1, 1, 4), (2, 0, 4), (1, 3, 1)):
+        for strides in itertools.product((0, 1, 2, 4, 5, 8, 12, 15, 24), repeat=len(shape)):
+            t = base.as_strided(shape, strides)
+            if rows_in_place(t):
+                taken += 1
+                assert readable(t), (shape, strides)
+    assert taken > 100
