@@ -3,7 +3,7 @@ formulas.  Bounds are that file's, which count roundings."""
 import pytest
 import torch
 
-from test_gpu_block import BF, D, F32, check_distill, check_linear, rnd, teacher_rows
+from test_gpu_block import BF, D, F32, check_distill, check_linear, close, rnd, teacher_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,81 @@ def test_distill_a_single_row_of_any_stride(amd, dtype):
         ids, teacher, lse = teacher_rows(1, 1, V, K, 1.0 if tail else None)
         for i, logits in enumerate(single_rows(50, V, dtype)):
             check_distill(amd, logits, ids, teacher, lse, None, 1.0, None, (i, tail))
+
+
+def capped64(logits, ids, teacher, lse, cap, tau, up):
+    """losses and gradient with their bounds, for lists of distinct columns; cap[0] / tau and |logits| are moderate"""
+    A, B, C = cap
+    l = logits.double()
+    s = torch.sigmoid((l + B) / C)
+    z = A * s / tau
+    logq = z - torch.logsumexp(z, 1, keepdim=True)
+    q = logq.exp()
+    t = teacher.double() / tau
+    logp = t - (torch.logsumexp(t, 1) if lse is None else lse.double())[:, None]
+    p = logp.exp()
+    loss = (p * (logp - logq.gather(1, ids))).sum(1)
+    sum_p = p.sum(1)
+    rest, ratio, log_others = torch.zeros_like(sum_p), torch.zeros_like(sum_p), torch.zeros_like(sum_p)
+    if lse is not None and ids.shape[1] < logits.shape[1]:
+        rest = (1 - sum_p).clamp_min(0)
+        log_others = logq.scatter(1, ids, -torch.inf).logsumexp(1)
+        loss = loss + rest * (rest.log() - log_others)
+        ratio = rest / log_others.exp()
+    listed = torch.zeros_like(q).scatter(1, ids, 1.0)
+    pv = torch.zeros_like(q).scatter(1, ids, p)
+    f = (sum_p + rest)[:, None] - ratio[:, None] * (1 - listed)
+    slope = A / C * s * (1 - s)
+    base = (tau * up.double())[:, None]
+    # Roundings E of a term: its exponent of |k1 l + k0| < 6 to 12 E, sigma then to 13 E, times A / tau, and the exponential's own 2 E.  Sums: 56
+    # values a thread, 24 levels of a tree; places of -inf that are subtracted again (at most 7 beside the row, or the listed columns, each the
+    # smallest term there is) weigh 8 times as much.  The loss takes each sum twice and the listed columns' exponents once more.
+    E = 2.0 ** -24
+    rel = (26 * A / tau + 160) * E
+    size = 1 + (p * logp.abs()).sum(1) + (p * (z.gather(1, ids) - z.gather(1, ids).max(1, keepdim=True)[0]).abs()).sum(1) + rest * log_others.abs()
+    lbound = tau * tau * (rel * (sum_p + 2 * rest) + 8 * E * size)
+    grad = base * (q * f - pv) * slope
+    fabs = (sum_p + rest + ratio)[:, None]
+    gbound = base.abs() * ((q * fabs * 3 * rel + pv * 8 * E) * slope + (q * fabs + pv) * 16 * E * A / C * s) + (2.0 ** -8 if logits.dtype == BF else E) * grad.abs()
+    return (tau * tau * loss, lbound), (grad, gbound)
+
+
+@pytest.mark.parametrize("dtype", [BF, F32])
+@pytest.mark.parametrize("tail", [False, True], ids=["list", "rest"])
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 9, 57, 100, 256, 1003, 16401])
+def test_distill_with_a_small_cap(amd, dtype, tail, V):
+    """the cap's smallest term is no longer negligible: what is read outside a row, or of listed columns, must not reach its sum"""
+    for T in (3, 600):                                   # no more rows than compute units, and more
+        for i, (A, tau) in enumerate(((0.5, 1.0), (1.0, 1.0), (4.0, 2.0), (5.0, 1.0))):
+            cap = (A, 5.0, 7.5)
+            for K in {1, min(max(1, V // 3), 512), min(V - 1, 512) or 1}:
+                ids, teacher, lse = teacher_rows(V + i, 8, V, K, tau if tail else None)
+                rows = lambda t: None if t is None else t.repeat(T // 8 + 1, *[1] * (t.ndim - 1))[:T].contiguous()
+                logits = rows(rnd(V + i + 1, 8, V, dtype=dtype, scale=3.0))
+                ids, teacher, lse = rows(ids), rows(teacher), rows(lse)
+                up = torch.rand(T, generator=torch.Generator().manual_seed(i)).to(D) + 0.5
+                what = (V, T, A, tau, K)
+                loss, grad = capped64(logits, ids, teacher, lse, cap, tau, up)
+                kw = dict(teacher_lse=lse, temperature=tau, softcap=cap)
+                leaf = logits.clone().requires_grad_()
+                got = amd.distill_topk(leaf, ids, teacher, **kw)
+                close(got.detach(), *loss, (what, "loss"))
+                close(torch.autograd.grad(got, [leaf], up)[0], *grad, (what, "grad"))
+                fused = amd.distill_topk_fwd_bwd(logits, ids, teacher, grad_scale=0.25, **kw)
+                close(fused[0], *loss, (what, "fused loss"))
+                close(fused[1], *capped64(logits, ids, teacher, lse, cap, tau, torch.full((T,), 0.25, device=D))[1], (what, "fused grad"))
+
+
+def test_distill_with_a_small_cap_on_rows_that_start_anywhere(amd):
+    T, V, K = 5, 39, 3
+    for dtype in (BF, F32):
+        big = rnd(2, T, V + 29, dtype=dtype, scale=3.0)
+        for tail in (False, True):
+            ids, teacher, lse = teacher_rows(1, T, V, K, 1.0 if tail else None)
+            for off in range(9):
+                logits = big[:, off:off + V]
+                up = torch.full((T,), 0.25, device=D)
+                loss, grad = capped64(logits, ids, teacher, lse, (1.0, 5.0, 7.5), 1.0, up)
+                got = amd.distill_topk_fwd_bwd(logits, ids, teacher, teacher_lse=lse, softcap=(1.0, 5.0, 7.5), grad_scale=0.25)
+                close(got[0], *loss, (off, "loss"))
+                close(got[1], *grad, (off, "grad"))
