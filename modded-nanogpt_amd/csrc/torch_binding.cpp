@@ -33,13 +33,16 @@ void check(int code, const char* what) {
     if (code != 0) TORCH_CHECK(false, what, " failed with code ", code, ": ", ngpt_last_error());
 }
 
-// Memory on that GPU (the wrappers of torch.func have none).
-bool on_gpu(const Tensor& t, const Tensor& like) { return !t.defined() || (t.is_cuda() && t.has_storage() && t.device() == like.device()); }
-bool wants_grad(const Tensor& t) {
-    if (!t.defined()) return false;
-    TORCH_CHECK(!t._fw_grad(0).defined(), "nanogpt operators have no forward-mode derivative");
-    return t.requires_grad();
+// A tensor that carries a forward-mode derivative is refused wherever it comes in: such derivatives do not go by the grad mode.
+const Tensor& no_tangent(const Tensor& t) {
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "nanogpt operators have no forward-mode derivative");
+    return t;
 }
+// Memory on that GPU (the wrappers of torch.func have none).
+bool on_gpu(const Tensor& t, const Tensor& like) {
+    return !t.defined() || (t.is_cuda() && t.has_storage() && t.device() == like.device() && no_tangent(t).defined());
+}
+bool wants_grad(const Tensor& t) { return t.defined() && t.requires_grad(); }
 
 Tensor workspace(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : Tensor(); }
 
@@ -99,7 +102,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& grad, const Ten
                                                    bool need_dw, bool need_db) {
     const c10::DeviceGuard guard(x.device());
     const Rows xr(x), wr(w);
-    const Tensor dout = grad.contiguous();
+    const Tensor dout = no_tangent(grad).contiguous();
     Tensor dx = need_dx ? at::empty(x.sizes(), x.options()) : Tensor(), dw = need_dw ? at::empty(w.sizes(), w.options()) : Tensor();
     Tensor db = need_db ? at::empty({wr.n}, w.options()) : Tensor();
     if (need_dx || need_dw || need_db) {
@@ -238,7 +241,7 @@ std::tuple<Tensor, Tensor> rope_forward(const RopeCall& c, const Tensor& q, cons
     return {qo, ko};
 }
 
-Tensor unit_stride(const Tensor& t) { return t.stride(-1) == 1 ? t : t.contiguous(); }
+Tensor unit_stride(const Tensor& t) { return no_tangent(t).stride(-1) == 1 ? t : t.contiguous(); }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> rope_backward(const RopeCall& c, const Tensor& gq, const Tensor& gk, const Tensor& q, const Tensor& k, const Tensor& cos,
                                                          const Tensor& sin, const Tensor& pos, const Tensor& qw, const Tensor& kw, double eps,
@@ -352,7 +355,7 @@ Tensor distill_backward(const Tensor& dlosses, const Tensor& logits, const Tenso
                         const Tensor& stats, const DistillParams& p) {
     const c10::DeviceGuard guard(logits.device());
     Tensor grad = at::empty(logits.sizes(), logits.options());
-    check(ngpt_distill_bwd(DISTILL_ARGS, (const float*)ptr(stats), (const float*)ptr(dlosses), dlosses.stride(0), out_ptr(grad), logits.size(1),
+    check(ngpt_distill_bwd(DISTILL_ARGS, (const float*)ptr(stats), (const float*)ptr(no_tangent(dlosses)), dlosses.stride(0), out_ptr(grad), logits.size(1),
                            stream_of(logits)), "ngpt_distill_bwd");
     return grad;
 }

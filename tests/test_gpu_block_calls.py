@@ -119,3 +119,59 @@ def test_distill_with_a_small_cap_on_rows_that_start_anywhere(amd):
                 got = amd.distill_topk_fwd_bwd(logits, ids, teacher, teacher_lse=lse, softcap=(1.0, 5.0, 7.5), grad_scale=0.25)
                 close(got[0], *loss, (off, "loss"))
                 close(got[1], *grad, (off, "grad"))
+
+
+def every_call(amd):
+    """(name, function, its tensors) of the four functions with every tensor that they take"""
+    M, K, N, V, C = 12, 64, 72, 300, 5
+    from test_gpu_block import tables
+    cos, sin = tables(M, 24)
+    ids, teacher, lse = teacher_rows(5, M, V, C, 1.0)
+    weight = torch.rand(M, generator=torch.Generator().manual_seed(1)).to(D)
+    yield "linear_act", lambda x, w, b, r: amd.linear_act(x, w, b, r, "gelu"), [rnd(1, M, K), rnd(2, N, K, scale=0.1), rnd(3, N), rnd(4, M, N)]
+    yield "qk_norm_rope", lambda q, k, c, s, g, h: amd.qk_norm_rope(q, k, c, s, None, g, h), [rnd(6, M, 4, 24), rnd(7, M, 2, 24), cos, sin, rnd(8, 24), rnd(9, 24)]
+    yield "distill_topk", lambda l, t, e, w: amd.distill_topk(l, ids, t, e, w), [rnd(10, M, V), teacher, lse, weight]
+    yield "distill_topk_fwd_bwd", lambda l, t, e, w: amd.distill_topk_fwd_bwd(l, ids, t, e, w), [rnd(10, M, V), teacher, lse, weight]
+
+
+def test_forward_mode_is_refused_for_every_tensor_in_every_mode(amd):
+    from torch.autograd import forward_ad
+    for name, f, tensors in every_call(amd):
+        for i, t in enumerate(tensors):
+            for spread in (False, True):                       # in usable form, and one that is copied first
+                for mode in (torch.no_grad(), torch.enable_grad()):
+                    with forward_ad.dual_level(), mode:
+                        if spread:
+                            base = torch.empty(*t.shape, 2, dtype=t.dtype, device=D)
+                            dual = forward_ad.make_dual(base.copy_(t.unsqueeze(-1)), torch.ones_like(base))[..., 0]
+                        else:
+                            dual = forward_ad.make_dual(t, torch.ones_like(t))
+                        args = [dual if j == i else u for j, u in enumerate(tensors)]
+                        with pytest.raises(RuntimeError, match="forward-mode"):
+                            f(*args)
+
+
+def test_forward_mode_is_refused_by_the_registered_operators(amd):
+    from torch.autograd import forward_ad
+    ops = torch.ops.nanogpt
+    (_, _, lin), (_, _, rope), (_, _, dist), _ = every_call(amd)
+    ids = teacher_rows(5, 12, 300, 5)[0]
+    calls = [(lambda x: ops.linear_act(x, lin[1], None, None, "none", False), lin[0]),
+             (lambda q: ops.qk_norm_rope(q, *rope[1:4], None, None, None, 1e-6, False), rope[0]),
+             (lambda l: ops.distill_topk(l, ids, dist[1], None, None, 1.0, 0.0, 0.0, 0.0), dist[0]),
+             (lambda l: ops.distill_topk_fwd_bwd(l, ids, dist[1], None, None, 1.0, 0.0, 0.0, 0.0, 1.0), dist[0])]
+    for f, t in calls:
+        with forward_ad.dual_level(), torch.no_grad(), pytest.raises(RuntimeError, match="forward-mode"):
+            f(forward_ad.make_dual(t, torch.ones_like(t)))
+
+
+def test_a_forward_mode_incoming_gradient_is_refused(amd):
+    from torch.autograd import forward_ad
+    for name, f, tensors in every_call(amd):
+        if name == "distill_topk_fwd_bwd":
+            continue
+        leaf = tensors[0].clone().requires_grad_()
+        out = f(leaf, *tensors[1:])
+        out = out if torch.is_tensor(out) else out[0]
+        with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
+            torch.autograd.grad(out, [leaf], forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
