@@ -147,6 +147,8 @@ def _linear_backward(ctx, dout, _dpre):
     if dout is None:
         return None, None, None, None, None, None
     need = ctx.needs_input_grad
+    if not any(need[:3]):               # the residual alone: there is no pre-activation then
+        return None, None, None, dout, None, None
     dx, dw, db = torch.ops.nanogpt.linear_act_backward(dout, x, w, pre, ctx.activation, need[0], need[1], need[2])
     return (dx if need[0] else None, dw if need[1] else None, db if need[2] else None, dout if need[3] else None, None, None)
 

@@ -175,3 +175,22 @@ def test_a_forward_mode_incoming_gradient_is_refused(amd):
         out = out if torch.is_tensor(out) else out[0]
         with forward_ad.dual_level(), pytest.raises(RuntimeError, match="forward-mode"):
             torch.autograd.grad(out, [leaf], forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out)))
+
+
+def test_linear_act_gradient_of_the_residual_alone(amd):
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Pass(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    x, w, b, dout = rnd(1, 9, 64), rnd(2, 24, 64), rnd(3, 24), rnd(4, 9, 24)
+    for act in ("none", "gelu"):
+        r = rnd(5, 9, 24).requires_grad_()
+        f = lambda r: amd.linear_act(x, w, b, r, act)
+        (eager,) = torch.autograd.grad(f(r), [r], dout)
+        with Pass():
+            (mode,) = torch.autograd.grad(f(r), [r], dout)
+        (traced,) = torch.autograd.grad(torch.compile(f, backend="aot_eager", fullgraph=True, dynamic=False)(r), [r], dout)
+        for g in (eager, mode, traced):
+            assert torch.equal(g, dout), act
