@@ -352,7 +352,10 @@ int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* w_bf16, int
 /* Its gradients from dout [M, N] (contiguous; it is the residual's gradient itself): dz = bf16(dout act'(pre)), dx [M, K] = dz w,
  * dw [N, K] = dz^T x, dbias [N] = sum of dout act'(pre) over the rows.  Each of the three outputs is nullable; pre may be null for
  * NGPT_ACT_NONE, w without dx, x without dw. */
-int64_t ngpt_linear_act_bwd_workspace_bytes(int M, int N, int K);
+int64_t ngpt_linear_act_bwd_workspace_bytes(int M, int N, int K);      /* the most that any call of these sizes uses */
+/* what one call uses on the current device, by which outputs are wanted and how dout and x lie in memory (0: the workspace may be null) */
+int64_t ngpt_linear_act_bwd_workspace_bytes_for(const void* dout_bf16, const void* x_bf16, int64_t ldx, int M, int N, int K, int activation,
+                                                int want_dx, int want_dw, int want_dbias);
 int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw,
                         int M, int N, int K, int activation, void* dx_bf16, void* dw_bf16, void* dbias_bf16,
                         void* workspace, int64_t workspace_bytes, void* stream);

@@ -76,6 +76,7 @@ SIGNATURES = {
                                       _F, _F, _F, _P, _P, _I, _P, _L, _P]),
     "ngpt_linear_act_fwd": (_I, [_P, _L, _P, _L, _P, _P, _L, _I, _I, _I, _I, _P, _P, _P]),
     "ngpt_linear_act_bwd_workspace_bytes": (_L, [_I, _I, _I]),
+    "ngpt_linear_act_bwd_workspace_bytes_for": (_L, [_P, _P, _L, _I, _I, _I, _I, _I, _I, _I]),
     "ngpt_linear_act_bwd": (_I, [_P, _P, _P, _L, _P, _L, _I, _I, _I, _I, _P, _P, _P, _P, _L, _P]),
     "ngpt_qk_norm_rope": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P, _I, _I, _P, _I, _P, _P, _P, _F, _I, _P, _P, _P]),
     "ngpt_qk_norm_rope_bwd_workspace_bytes": (_L, [_I]),

@@ -167,6 +167,12 @@ int64_t balanced_part_bytes(int R, int C, int K) {
     return parts * MainCfg::BM * MainCfg::BN * 4;
 }
 
+// The same on the current device, for exactly this product.
+int64_t balanced_part_bytes_here(int R, int C, int K) {
+    const BalancePlan p = plan_balance(R, C, K);
+    return p.splits > 1 ? (int64_t)p.rem * p.splits * MainCfg::BM * MainCfg::BN * 4 : 0;
+}
+
 // C[R, C] = scale * A . B^T with the balanced walk.  `layout`: kBlockedA | kBlockedB.
 // part32: balanced_part_bytes(R, C, K) bytes of scratch for the split tiles.
 // fa may carry FMT_TRANSPOSED (A = panel of the transpose, a_rows_pad = R rounded up to 256).

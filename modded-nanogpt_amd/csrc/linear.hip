@@ -13,6 +13,7 @@
 namespace ngpt {
 // gemm_api.hip
 int64_t balanced_part_bytes(int R, int C, int K);
+int64_t balanced_part_bytes_here(int R, int C, int K);
 int gemm_bf16_clipped(const void* A, int fa, int64_t lda, const void* B, int fb, int64_t ldb, int R, int C, int K, int R_out, int C_out,
                       void* out_bf16, int64_t ldc, float* part32, hipStream_t st);
 
@@ -251,20 +252,35 @@ extern "C" int ngpt_linear_act_fwd(const void* x_bf16, int64_t ldx, const void* 
 
 namespace ngpt {
 namespace {
-// Workspace of the backward: dz [M64, N64] | w^T [K, N64] | x [M64, K8] (a copy where dw's product cannot read x in place) | parts of dw's split
-// tiles | column sums
+// Workspace of the backward: dz [M64, N64] | w^T [K, N64] | x [M64, K8] | parts of dw's split tiles | column sums, each of them where the
+// call has a use for it.
 struct BwdPlan {
     int64_t M64, N64, K8, dz, w, x, parts, sums, total;
     int sum_rows;
-    BwdPlan(int M, int N, int K) {
+    bool own_dz;      // dz is dout itself where there is no activation and the products can read it in place
+    bool copy_x;      // where dw's product cannot read x in place
+    // the most that a call of these sizes can use, on any device
+    BwdPlan(int M, int N, int K) : own_dz(true), copy_x(true) {
+        lay_out(M, N, K, true, true, balanced_part_bytes((int)up64(N), (int)up8(K), (int)(2 * up64(M))));
+    }
+    // one call on the current device
+    BwdPlan(int M, int N, int K, int act, const void* dout, const void* x_, int64_t ldx, bool dx, bool dw, bool dbias) {
+        own_dz = (dx || dw) && (act != NGPT_ACT_NONE || !on16(dout) || (dw && (M % 64 || N % 8)));
+        copy_x = dw && (M % 64 || K % 8 || ldx % 8 || !on16(x_));
+        // (rows of dw that are not whole groups of four are written without split tiles)
+        lay_out(M, N, K, dx, dbias, dw && K % 4 == 0 ? balanced_part_bytes_here(own_dz ? (int)up64(N) : N, (int)up8(K), (int)(2 * up64(M))) : 0);
+    }
+
+private:
+    void lay_out(int M, int N, int K, bool dx, bool dbias, int64_t part_bytes) {
         M64 = up64(M); N64 = up64(N); K8 = up8(K);
         dz = 0;
-        w = dz + align_up(M64 * N64 * 2, 256);
-        x = w + align_up(N64 * K * 2, 256);
-        parts = x + align_up(M64 * K8 * 2, 256);
-        sums = parts + align_up(balanced_part_bytes((int)N64, (int)K8, (int)(2 * M64)), 256);
+        w = dz + (own_dz ? align_up(M64 * N64 * 2, 256) : 0);
+        x = w + (dx ? align_up(N64 * K * 2, 256) : 0);
+        parts = x + (copy_x ? align_up(M64 * K8 * 2, 256) : 0);
+        sums = parts + align_up(part_bytes, 256);
         sum_rows = act_grad_rows(M, N);
-        total = sums + align_up((int64_t)sum_rows * N * 4, 256);
+        total = sums + (dbias ? align_up((int64_t)sum_rows * N * 4, 256) : 0);
     }
 };
 }  // namespace
@@ -273,6 +289,12 @@ struct BwdPlan {
 extern "C" int64_t ngpt_linear_act_bwd_workspace_bytes(int M, int N, int K) {
     if (M <= 0 || N <= 0 || K <= 0 || M > (1 << 29) || N > kMaxStride || K > kMaxStride) return 0;
     return BwdPlan(M, N, K).total;
+}
+
+extern "C" int64_t ngpt_linear_act_bwd_workspace_bytes_for(const void* dout_bf16, const void* x_bf16, int64_t ldx, int M, int N, int K, int activation,
+                                                           int want_dx, int want_dw, int want_dbias) {
+    if (ngpt_linear_act_bwd_workspace_bytes(M, N, K) == 0) return 0;
+    return BwdPlan(M, N, K, activation, dout_bf16, x_bf16, ldx, want_dx != 0, want_dw != 0, want_dbias != 0).total;
 }
 
 extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, const void* x_bf16, int64_t ldx, const void* w_bf16, int64_t ldw,
@@ -285,13 +307,12 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
     if ((dw_bf16 && ldx < K) || (dx_bf16 && ldw < K)) return fail(NGPT_EALIGN, "%s: row strides ldx=%lld ldw=%lld", who, (long long)ldx, (long long)ldw);
     if ((dw_bf16 && ldx > kMaxStride) || (dx_bf16 && ldw > kMaxStride))
         return fail(NGPT_ERANGE, "%s: row strides of at most 2^21 values (ldx=%lld ldw=%lld)", who, (long long)ldx, (long long)ldw);
-    const BwdPlan p(M, N, K);
-    if (!workspace || workspace_bytes < p.total || !on16(workspace))
+    const BwdPlan p(M, N, K, activation, dout_bf16, x_bf16, ldx, dx_bf16 != nullptr, dw_bf16 != nullptr, dbias_bf16 != nullptr);
+    if (p.total > 0 && (!workspace || workspace_bytes < p.total || !on16(workspace)))
         return fail(NGPT_EWORKSPACE, "%s: workspace %lld < %lld bytes", who, (long long)workspace_bytes, (long long)p.total);
     hipStream_t st = (hipStream_t)stream;
     uint8_t* ws = (uint8_t*)workspace;
-    // dz is dout itself where there is no activation and the products can read it in place
-    const bool own_dz = (dx_bf16 || dw_bf16) && (activation != NGPT_ACT_NONE || !on16(dout_bf16) || (dw_bf16 && (M % 64 || N % 8)));
+    const bool own_dz = p.own_dz;
     const uint16_t* dz = own_dz ? (const uint16_t*)(ws + p.dz) : (const uint16_t*)dout_bf16;
     const int64_t ld_dz = own_dz ? p.N64 : N;
     if (own_dz || dbias_bf16) {
@@ -321,7 +342,7 @@ extern "C" int ngpt_linear_act_bwd(const void* dout_bf16, const void* pre_bf16, 
     }
     if (dw_bf16) {      // dw [N, K] = dz^T . x, contraction over the M rows of both
         const void* x = x_bf16;
-        if (M % 64 || K % 8 || ldx % 8 || !on16(x)) {
+        if (p.copy_x) {
             if (int e = pad_copy(x_bf16, ldx, M, K, ws + p.x, p.M64, p.K8, st)) return e;
             x = ws + p.x;
             ldx = p.K8;

@@ -106,9 +106,10 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& grad, const Ten
     Tensor dx = need_dx ? at::empty(x.sizes(), x.options()) : Tensor(), dw = need_dw ? at::empty(w.sizes(), w.options()) : Tensor();
     Tensor db = need_db ? at::empty({wr.n}, w.options()) : Tensor();
     if (need_dx || need_dw || need_db) {
-        const Tensor ws = workspace(ngpt_linear_act_bwd_workspace_bytes((int)xr.n, (int)wr.n, (int)xr.len), x);
+        const Tensor ws = workspace(ngpt_linear_act_bwd_workspace_bytes_for(ptr(dout), ptr(x), xr.ld, (int)xr.n, (int)wr.n, (int)xr.len, (int)act, need_dx,
+                                                                            need_dw, need_db), x);
         check(ngpt_linear_act_bwd(ptr(dout), ptr(pre), ptr(x), xr.ld, ptr(w), wr.ld, (int)xr.n, (int)wr.n, (int)xr.len, (int)act, out_ptr(dx), out_ptr(dw),
-                                  out_ptr(db), out_ptr(ws), ws.numel(), stream_of(x)), "ngpt_linear_act_bwd");
+                                  out_ptr(db), out_ptr(ws), ws.defined() ? ws.numel() : 0, stream_of(x)), "ngpt_linear_act_bwd");
     }
     return {dx, dw, db};
 }

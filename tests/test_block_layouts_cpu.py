@@ -52,3 +52,25 @@ def test_what_is_read_in_place_is_where_the_kernels_look(rows_in_place):
                 taken += 1
                 assert readable(t), (shape, strides)
     assert taken > 100
+
+
+def test_the_backward_of_linear_act_reserves_what_it_uses():
+    import modded_nanogpt_amd
+    lib = modded_nanogpt_amd._lib.load()
+    M, N, K = 4096, 768, 768
+    need = lambda act=0, dout=16, x=16, ldx=K, dx=1, dw=1, db=1, M=M: lib.ngpt_linear_act_bwd_workspace_bytes_for(dout, x, ldx, M, N, K, act, dx, dw, db)
+    dz, wt, xc, most = 2 * M * N, 2 * N * K, 2 * M * K, lib.ngpt_linear_act_bwd_workspace_bytes(M, N, K)
+    assert need(db=0, dw=0) == wt and need(dx=0, dw=0) < 2048 * 4 * N + 256          # nothing but w^T; nothing but column sums
+    assert need(dx=0, dw=0, db=0) == 0
+    assert need(act=1, dw=0, db=0) == dz + wt and need(dout=8, dw=0, db=0) == dz + wt
+    parts = need(dx=0, db=0)                                                         # (by the device: none without one)
+    assert need(dx=0, db=0, x=8) == xc + parts == need(dx=0, db=0, ldx=K + 4)
+    assert need(dx=0, db=0, M=M - 1) == dz + xc + lib.ngpt_linear_act_bwd_workspace_bytes_for(16, 16, K, M, N, K, 0, 0, 1, 0)
+    for act in (0, 3):
+        for flags in itertools.product((0, 1), repeat=3):
+            for dout, x in itertools.product((16, 2), repeat=2):
+                assert need(act, dout, x, K, *flags) <= most
+    assert lib.ngpt_linear_act_bwd_workspace_bytes_for(16, 16, 64, 0, 8, 64, 0, 1, 1, 1) == 0
+    # what is asked for is what is refused below
+    bwd = lambda nws, dx=16, dw=16, db=16: lib.ngpt_linear_act_bwd(16, None, 16, K, 16, K, M, N, K, 0, dx, dw, db, 16, nws, None)
+    assert bwd(need() - 1) == -3 and bwd(need(dw=0, db=0) - 1, dw=None, db=None) == -3

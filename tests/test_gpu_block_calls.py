@@ -194,3 +194,45 @@ def test_linear_act_gradient_of_the_residual_alone(amd):
         (traced,) = torch.autograd.grad(torch.compile(f, backend="aot_eager", fullgraph=True, dynamic=False)(r), [r], dout)
         for g in (eager, mode, traced):
             assert torch.equal(g, dout), act
+
+
+@pytest.mark.parametrize("M,N,K", [(128, 64, 64), (4096, 768, 768), (4032, 768, 760), (1000, 250, 333), (33, 72, 100)])
+def test_linear_act_backward_stays_inside_its_workspace(amd, M, N, K):
+    """every combination of wanted outputs and layouts with the bytes that the query names, between two marked areas; the same bits as with plenty"""
+    import itertools
+    lib, stream = amd._lib.load(), torch.cuda.current_stream().cuda_stream
+    w, mark, guard = rnd(2, N, K, scale=0.1), 0xA5, 1 << 16
+    for act, off_d, off_x in itertools.product((0, 3), (0, 1), (0, 1)):
+        dout, x, pre = rnd(3, M * N + 8)[off_d:off_d + M * N], rnd(1, M * K + 8)[off_x:off_x + M * K], rnd(4, M, N) if act else None
+        ptr = lambda t: None if t is None else t.data_ptr()
+
+        def call(want, ws, n):
+            outs = [torch.empty(*s, dtype=BF, device=D) if k else None for k, s in zip(want, ((M, K), (N, K), (N,)))]
+            code = lib.ngpt_linear_act_bwd(ptr(dout), ptr(pre), ptr(x), K, ptr(w), K, M, N, K, act, *map(ptr, outs), ws, n, stream)
+            assert code == 0, (code, lib.ngpt_last_error())
+            return outs
+
+        most = lib.ngpt_linear_act_bwd_workspace_bytes(M, N, K)
+        plenty = torch.empty(most, dtype=torch.uint8, device=D)
+        want_all = call((1, 1, 1), plenty.data_ptr(), most)
+        for want in itertools.product((0, 1), repeat=3):
+            n = lib.ngpt_linear_act_bwd_workspace_bytes_for(ptr(dout), ptr(x), K, M, N, K, act, *want)
+            assert n <= most
+            area = torch.full((n + 2 * guard,), mark, dtype=torch.uint8, device=D)
+            outs = call(want, area.data_ptr() + guard if n else None, n)
+            assert (area[:guard] == mark).all() and (area[guard + n:] == mark).all(), (act, off_d, off_x, want)
+            for a, b in zip(outs, want_all):
+                assert a is None or torch.equal(a, b), (act, off_d, off_x, want)
+
+
+def test_linear_act_backward_memory(amd):
+    """a projection without an activation reads dout and x in place: beside its results it needs w^T and the parts of split tiles"""
+    M, N, K = 49152, 768, 768
+    x, w, dout = rnd(1, M, K).requires_grad_(), rnd(2, N, K, scale=0.1).requires_grad_(), rnd(3, M, N)
+    out = amd.linear_act(x, w)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    dx, dw = torch.autograd.grad(out, [x, w], dout)
+    extra = torch.cuda.max_memory_allocated() - before - (M + N) * K * 2
+    assert extra < 80 << 20, extra          # 1.2 MB and at most one 256 KiB part a compute unit (64 MiB); dz and a copy of x would be 151 MB
