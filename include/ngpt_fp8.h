@@ -42,6 +42,8 @@ extern "C" {
 #define NGPT_DT_BF16       0     /* element types of the operators that take more than one */
 #define NGPT_DT_F32        1
 
+#define NGPT_LINEAR_MAX_STRIDE (1 << 21)   /* ngpt_linear_act_*: most values between two rows, and in one */
+
 #define NGPT_ACT_NONE      0     /* activations of ngpt_linear_act: z */
 #define NGPT_ACT_RELU2     1     /* max(z, 0)^2 */
 #define NGPT_ACT_GELU      2     /* z Phi(z), Phi the normal distribution function */

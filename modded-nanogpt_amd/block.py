@@ -48,9 +48,9 @@ def _plain(*tensors: Tensor | None) -> bool:
     return True
 
 
-def _rows(t: Tensor | None) -> Tensor | None:
-    """[..., K] whose rows are contiguous, evenly spaced and do not overlap: itself, or a copy."""
-    return t if t is None or t.ndim == 0 or _b().rows_in_place(t) else t.contiguous()
+def _rows(t: Tensor | None, *most: int) -> Tensor | None:
+    """[..., K] whose rows are contiguous, evenly spaced (at most `most` values apart) and do not overlap: itself, or a copy."""
+    return t if t is None or t.ndim == 0 or _b().rows_in_place(t, *most) else t.contiguous()
 
 
 def _direct(*tensors: Tensor | None) -> bool:
@@ -88,7 +88,8 @@ def _linear_usable(x, w, bias, residual):
     """The same values in a form the kernels read in place (these copies are differentiable)."""
     if bias is not None and (not bias.is_contiguous() or bias.data_ptr() % 16):
         bias = bias.clone(memory_format=torch.contiguous_format)
-    return _rows(x), _rows(w), bias, _rows(residual)
+    most = _b().LINEAR_MAX_STRIDE
+    return _rows(x, most), _rows(w, most), bias, _rows(residual, most)
 
 
 @torch.library.custom_op("nanogpt::linear_act", mutates_args=())

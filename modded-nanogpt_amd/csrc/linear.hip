@@ -173,7 +173,7 @@ int act_grad_rows(int64_t M, int64_t N) {
     return (int)std::max<int64_t>(rows, 1);
 }
 
-constexpr int64_t kMaxStride = 1 << 21;      // values between rows: 256 rows of a tile lie within 32-bit byte offsets
+constexpr int64_t kMaxStride = NGPT_LINEAR_MAX_STRIDE;      // values between rows: 256 rows of a tile lie within 32-bit byte offsets
 
 int check_linear(const char* who, int M, int N, int K, int act) {
     if (M <= 0 || N <= 0 || K <= 0) return fail(NGPT_EINVAL, "%s: empty problem M=%d N=%d K=%d", who, M, N, K);

@@ -51,7 +51,7 @@ Tensor workspace(int64_t bytes, const Tensor& like) { return bytes > 0 ? at::emp
 struct Rows {
     int64_t n = 0, len = 0, ld = 0;
     bool ok = false;
-    explicit Rows(const Tensor& t) {
+    explicit Rows(const Tensor& t, int64_t most = INT64_MAX) {      // `most`: the longest distance between rows that can be read in place
         const int64_t d = t.dim();
         if (d < 1) return;
         len = t.size(d - 1);
@@ -62,7 +62,7 @@ struct Rows {
         ok = n <= 1;
         if (ok) return;
         ld = d > 1 ? t.stride(d - 2) : 0;
-        ok = ld >= len;
+        ok = ld >= len && ld <= most;
         for (int64_t i = 0; i + 2 < d; ++i) ok = ok && t.stride(i) == t.stride(i + 1) * t.size(i + 1);      // one stride for all rows
     }
 };
@@ -76,11 +76,11 @@ bool linear_usable(const Tensor& x, const Tensor& w, const Tensor& bias, const T
     if (w.dim() != 2 || x.dim() < 1 || x.size(-1) != w.size(1)) return false;
     for (const Tensor* t : {&x, &w, &bias, &residual})
         if (t->defined() && t->scalar_type() != at::kBFloat16) return false;
-    const Rows xr(x), wr(w);
+    const Rows xr(x, NGPT_LINEAR_MAX_STRIDE), wr(w, NGPT_LINEAR_MAX_STRIDE);
     if (!xr.ok || !wr.ok || xr.n == 0 || wr.n == 0 || xr.len == 0 || xr.n > kInt || wr.n > kInt || xr.len > kInt) return false;
     if (bias.defined() && (bias.dim() != 1 || bias.size(0) != wr.n || !bias.is_contiguous() || ((uintptr_t)bias.const_data_ptr() & 15))) return false;
     if (residual.defined()) {
-        if (residual.dim() != x.dim() || residual.size(-1) != wr.n || !Rows(residual).ok) return false;
+        if (residual.dim() != x.dim() || residual.size(-1) != wr.n || !Rows(residual, NGPT_LINEAR_MAX_STRIDE).ok) return false;
         for (int64_t i = 0; i + 1 < x.dim(); ++i)
             if (residual.size(i) != x.size(i)) return false;
     }
@@ -517,7 +517,9 @@ PyMethodDef methods[] = {method<py_linear_act>("linear_act"), method<py_qk_norm_
 
 PYBIND11_MODULE(_ngpt_torch, m) {
     if (PyModule_AddFunctions(m.ptr(), methods) != 0) throw pybind11::error_already_set();
-    m.def("rows_in_place", [](const Tensor& t) { return Rows(t).ok; });      // the one rule for Python's copies too; looks at sizes and strides only
+    // the one rule for Python's copies too; looks at sizes and strides only
+    m.def("rows_in_place", [](const Tensor& t, int64_t most) { return Rows(t, most).ok; }, pybind11::arg("t"), pybind11::arg("most") = INT64_MAX);
+    m.attr("LINEAR_MAX_STRIDE") = NGPT_LINEAR_MAX_STRIDE;
     m.def("linear_raw", &linear_raw);
     m.def("linear_backward_raw", &linear_backward_raw);
     m.def("rope_backward_raw", &rope_backward_raw);

@@ -74,3 +74,12 @@ def test_the_backward_of_linear_act_reserves_what_it_uses():
     # what is asked for is what is refused below
     bwd = lambda nws, dx=16, dw=16, db=16: lib.ngpt_linear_act_bwd(16, None, 16, K, 16, K, M, N, K, 0, dx, dw, db, 16, nws, None)
     assert bwd(need() - 1) == -3 and bwd(need(dw=0, db=0) - 1, dw=None, db=None) == -3
+
+
+def test_rows_too_far_apart_are_copied(rows_in_place):
+    import modded_nanogpt_amd
+    most = modded_nanogpt_amd._lib.load_torch().LINEAR_MAX_STRIDE
+    t = torch.empty(3, most + 64, device="meta")
+    assert rows_in_place(t[:, :64]) and not rows_in_place(t[:, :64], most) and rows_in_place(t[:1, :64], most)
+    assert rows_in_place(t, most)              # contiguous: a copy would not help
+    assert rows_in_place(t[:, 64:].new_empty(3, most)[:, 3:], most)

@@ -236,3 +236,13 @@ def test_linear_act_backward_memory(amd):
     dx, dw = torch.autograd.grad(out, [x, w], dout)
     extra = torch.cuda.max_memory_allocated() - before - (M + N) * K * 2
     assert extra < 80 << 20, extra          # 1.2 MB and at most one 256 KiB part a compute unit (64 MiB); dz and a copy of x would be 151 MB
+
+
+def test_linear_act_rows_far_apart(amd):
+    """x, w and residual of more than 2^21 values between rows: copied, like other layouts that cannot be read in place"""
+    M, N, K, far = 5, 24, 72, (1 << 21) + 8
+    spread = lambda seed, rows, n: torch.zeros(rows, far, dtype=BF, device=D)[:, 3:3 + n].copy_(rnd(seed, rows, n))
+    x, w, r = spread(1, M, K), spread(2, N, K), spread(3, M, N)
+    for i, (a, b, c) in enumerate(((x, w.contiguous(), None), (x.contiguous(), w, None), (x.contiguous(), w.contiguous(), r), (x, w, r))):
+        check_linear(amd, a, b, None, c, "gelu", rnd(4, M, N), i)
+    assert torch.equal(torch.ops.nanogpt.linear_act(x, w, None, r, "none", False)[0], amd.linear_act(x.contiguous(), w.contiguous(), None, r.contiguous()))
