@@ -61,9 +61,14 @@ struct Rows {
         if (ok || (len > 1 && t.stride(d - 1) != 1)) return;
         ok = n <= 1;
         if (ok) return;
-        ld = d > 1 ? t.stride(d - 2) : 0;
+        int64_t i = d - 2;
+        while (t.size(i) == 1) --i;                   // (n > 1: there is one)
+        ld = t.stride(i);
         ok = ld >= len && ld <= most;
-        for (int64_t i = 0; i + 2 < d; ++i) ok = ok && t.stride(i) == t.stride(i + 1) * t.size(i + 1);      // one stride for all rows
+        for (int64_t next = ld; i >= 0; --i) {        // where a dimension has to continue: one distance for all rows
+            ok = ok && (t.size(i) == 1 || t.stride(i) == next);
+            next *= t.size(i);
+        }
     }
 };
 

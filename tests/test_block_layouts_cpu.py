@@ -83,3 +83,11 @@ def test_rows_too_far_apart_are_copied(rows_in_place):
     assert rows_in_place(t[:, :64]) and not rows_in_place(t[:, :64], most) and rows_in_place(t[:1, :64], most)
     assert rows_in_place(t, most)              # contiguous: a copy would not help
     assert rows_in_place(t[:, 64:].new_empty(3, most)[:, 3:], most)
+
+
+def test_dimensions_of_size_one_do_not_make_rows_uneven(rows_in_place):
+    t = torch.zeros(4, 9, 6, 48)
+    for v in (t[:, -1:, 0], t[:, -1:, :1], t[:, :, :1, 5:20], t[:, -1, :1], t[:1, :, :1], t[:, :, :, 3:], t[:, 0, None, 2]):
+        assert readable(v) and rows_in_place(v), (v.shape, v.stride())
+    for v in (t[:, :2, 0], t[:, -1:, :, 3:], t[:, :1].expand(4, 3, 6, 48), t[:, :1, :5], t.transpose(0, 1)[:, :, :1]):
+        assert not rows_in_place(v), (v.shape, v.stride())

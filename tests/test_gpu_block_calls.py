@@ -246,3 +246,19 @@ def test_linear_act_rows_far_apart(amd):
     for i, (a, b, c) in enumerate(((x, w.contiguous(), None), (x.contiguous(), w, None), (x.contiguous(), w.contiguous(), r), (x, w, r))):
         check_linear(amd, a, b, None, c, "gelu", rnd(4, M, N), i)
     assert torch.equal(torch.ops.nanogpt.linear_act(x, w, None, r, "none", False)[0], amd.linear_act(x.contiguous(), w.contiguous(), None, r.contiguous()))
+
+
+def test_linear_act_last_position_of_every_sequence(amd):
+    """[B, 1, K] out of [B, T, K]: evenly spaced rows, read in place"""
+    B, T, N, K = 7, 5, 40, 96
+    h, r, w = rnd(1, B, T, K), rnd(2, B, T, N), rnd(3, N, K, scale=0.1)
+    x, res = h[:, -1:], r[:, -1:]
+    want = amd.linear_act(x.contiguous(), w, None, res.contiguous(), "silu")
+    before = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = amd.linear_act(x, w, None, res, "silu")
+    peak = torch.cuda.max_memory_allocated() - before          # (ahead of the comparison, which allocates)
+    assert torch.equal(got, want) and got.shape == (B, 1, N)
+    assert peak <= 512 * -(-B * N * 2 // 512)                  # the result, no copies
+    check = amd.linear_act(h[:, -1].requires_grad_(), w, None, r[:, -1], "silu")
+    assert torch.equal(check, want[:, 0])
