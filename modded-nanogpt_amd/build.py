@@ -1,12 +1,14 @@
 """Builds libngpt_fp8.so (all HIP kernels + the C ABI) for gfx950 with hipcc, in-tree, and the host-side torch binding beside it.
 
     python -m modded_nanogpt_amd.build          # from the repository root
+    python modded-nanogpt_amd/build.py          # where there is no torch: the library alone, for programs that use its C ABI
 
 hipcc cross-compiles without a GPU.  The library lands in modded-nanogpt_amd/lib/ so it travels
 with the source tree; nothing is installed into site-packages.
 """
 from __future__ import annotations
 
+import importlib.util
 import os
 import pathlib
 import shutil
@@ -70,7 +72,8 @@ def _binding_commands(obj: str, lib_dir: str) -> tuple[list[str], list[str]]:
 
 
 def build(verbose: bool = True, bench: bool = False) -> pathlib.Path:
-    """Compile every HIP source into one shared library; always recompiles.  `bench`: the measurement build."""
+    """Compile every HIP source into one shared library; always recompiles.  `bench`: the measurement build.
+    The torch binding needs torch and is left out where there is none; where it fails, the library is in place all the same."""
     LIB_DIR.mkdir(exist_ok=True)
     srcs = [str(CSRC / s) for s in SOURCES if (CSRC / s).exists()]
     out = BENCH_LIB_PATH if bench else LIB_PATH
@@ -78,16 +81,24 @@ def build(verbose: bool = True, bench: bool = False) -> pathlib.Path:
     flags = [*[f for f in HIPCC_FLAGS if f != "-shared"], *(["-DNGPT_BENCH_BUILD"] if bench else []), "-I", str(PKG.parent / "include")]
     with tempfile.TemporaryDirectory() as objdir:
         # one object a source, compiled side by side, then one link
-        binding = None if bench else _binding_commands(str(pathlib.Path(objdir) / "torch_binding.o"), str(LIB_DIR))
+        def compile_binding() -> list[str]:
+            compile_, link = _binding_commands(str(pathlib.Path(objdir) / "torch_binding.o"), str(LIB_DIR))
+            _run(compile_, verbose)
+            return link
+
         objs = [str(pathlib.Path(objdir) / (pathlib.Path(s).stem + ".o")) for s in srcs]
-        jobs = [[hipcc_path(), *flags, "-c", "-o", o, c] for c, o in zip(srcs, objs)] + ([binding[0]] if binding else [])
-        with ThreadPoolExecutor(max_workers=min(len(jobs), os.cpu_count() or 1, 8)) as pool:
+        jobs = [[hipcc_path(), *flags, "-c", "-o", o, c] for c, o in zip(srcs, objs)]
+        with_torch = not bench and importlib.util.find_spec("torch") is not None
+        with ThreadPoolExecutor(max_workers=min(len(jobs) + 1, os.cpu_count() or 1, 8)) as pool:
+            binding = pool.submit(compile_binding) if with_torch else None
             list(pool.map(lambda job: _run(job, verbose), jobs))
-        _run([hipcc_path(), *HIPCC_FLAGS, "-o", str(tmp), *objs], verbose)
-        os.replace(tmp, out)
-        if binding:
-            _run(binding[1], verbose)
-            os.replace(str(BINDING_PATH) + ".tmp", BINDING_PATH)
+            _run([hipcc_path(), *HIPCC_FLAGS, "-o", str(tmp), *objs], verbose)
+            os.replace(tmp, out)
+            if binding:
+                _run(binding.result(), verbose)
+                os.replace(str(BINDING_PATH) + ".tmp", BINDING_PATH)
+        if verbose and not bench and not with_torch:
+            print("no torch: the library without its torch binding", flush=True)
     return out
 
 
