@@ -39,11 +39,11 @@ def _same_gpu(first: Tensor, *others: Tensor | None) -> None:
 
 
 def _plain(*tensors: Tensor | None) -> bool:
-    """Ordinary tensors outside of a trace and of dispatch modes: the kernels can be launched here."""
+    """Ordinary tensors that hold their own values, outside of a trace and of dispatch modes: the kernels can be launched here."""
     if torch.compiler.is_compiling() or torch._C._len_torch_dispatch_stack() or torch._C._get_tracing_state() is not None:
         return False
     for t in tensors:
-        if t is not None and type(t) is not Tensor and type(t) is not torch.nn.Parameter:
+        if t is not None and (type(t) is not Tensor and type(t) is not torch.nn.Parameter or t.is_neg()):
             return False
     return True
 

@@ -107,7 +107,7 @@ std::tuple<Tensor, Tensor, Tensor> linear_backward(const Tensor& grad, const Ten
                                                    bool need_dw, bool need_db) {
     const c10::DeviceGuard guard(x.device());
     const Rows xr(x), wr(w);
-    const Tensor dout = no_tangent(grad).contiguous();
+    const Tensor dout = no_tangent(grad).contiguous().resolve_neg();
     Tensor dx = need_dx ? at::empty(x.sizes(), x.options()) : Tensor(), dw = need_dw ? at::empty(w.sizes(), w.options()) : Tensor();
     Tensor db = need_db ? at::empty({wr.n}, w.options()) : Tensor();
     if (need_dx || need_dw || need_db) {
@@ -247,7 +247,7 @@ std::tuple<Tensor, Tensor> rope_forward(const RopeCall& c, const Tensor& q, cons
     return {qo, ko};
 }
 
-Tensor unit_stride(const Tensor& t) { return no_tangent(t).stride(-1) == 1 ? t : t.contiguous(); }
+Tensor unit_stride(const Tensor& t) { return no_tangent(t).stride(-1) == 1 ? t.resolve_neg() : t.contiguous().resolve_neg(); }
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> rope_backward(const RopeCall& c, const Tensor& gq, const Tensor& gk, const Tensor& q, const Tensor& k, const Tensor& cos,
                                                          const Tensor& sin, const Tensor& pos, const Tensor& qw, const Tensor& kw, double eps,
@@ -357,11 +357,12 @@ std::tuple<Tensor, Tensor> distill_forward(const Tensor& logits, const Tensor& i
     return {losses, stats};
 }
 
-Tensor distill_backward(const Tensor& dlosses, const Tensor& logits, const Tensor& ids, const Tensor& teacher, const Tensor& lse, const Tensor& weight,
+Tensor distill_backward(const Tensor& grad_, const Tensor& logits, const Tensor& ids, const Tensor& teacher, const Tensor& lse, const Tensor& weight,
                         const Tensor& stats, const DistillParams& p) {
     const c10::DeviceGuard guard(logits.device());
+    const Tensor dlosses = no_tangent(grad_).resolve_neg();
     Tensor grad = at::empty(logits.sizes(), logits.options());
-    check(ngpt_distill_bwd(DISTILL_ARGS, (const float*)ptr(stats), (const float*)ptr(no_tangent(dlosses)), dlosses.stride(0), out_ptr(grad), logits.size(1),
+    check(ngpt_distill_bwd(DISTILL_ARGS, (const float*)ptr(stats), (const float*)ptr(dlosses), dlosses.stride(0), out_ptr(grad), logits.size(1),
                            stream_of(logits)), "ngpt_distill_bwd");
     return grad;
 }
@@ -439,7 +440,9 @@ struct Given {
             ok = false;
             return std::nullopt;
         }
-        return THPVariable_Unpack(o);
+        const Tensor& t = THPVariable_Unpack(o);
+        ok = ok && !t.is_neg();                             // memory that holds the negated values: the dispatcher makes them real
+        return t;
     }
     Tensor tensor(int i) {
         OptTensor t = maybe(i);

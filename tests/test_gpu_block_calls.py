@@ -262,3 +262,30 @@ def test_linear_act_last_position_of_every_sequence(amd):
     assert peak <= 512 * -(-B * N * 2 // 512)                  # the result, no copies
     check = amd.linear_act(h[:, -1].requires_grad_(), w, None, r[:, -1], "silu")
     assert torch.equal(check, want[:, 0])
+
+
+def test_lazily_negated_tensors(amd):
+    """the imaginary part of a conjugate shares its memory with the number and is negated when read"""
+    for name, f, tensors in every_call(amd):
+        tensors = [t.contiguous() for t in tensors]
+        for i, t in enumerate(tensors):
+            lazy = torch._neg_view((-t).contiguous())
+            assert lazy.is_neg() and lazy.is_contiguous()
+            got, want = f(*[lazy if j == i else u for j, u in enumerate(tensors)]), f(*tensors)
+            for a, b in zip(got if isinstance(got, tuple) else (got,), want if isinstance(want, tuple) else (want,)):
+                assert torch.equal(a, b), (name, i)
+        if name == "distill_topk_fwd_bwd":
+            continue
+        lazy = torch._neg_view((-tensors[0]).contiguous())
+        grads = []
+        for leaf in (tensors[0].detach().requires_grad_(), lazy.detach().requires_grad_()):
+            out = f(leaf, *tensors[1:])
+            out = out if torch.is_tensor(out) else out[0]
+            dout = rnd(3, *out.shape, dtype=out.dtype)
+            grads += [torch.autograd.grad(out, [leaf], d, retain_graph=True)[0] for d in (dout, torch._neg_view(-dout))]
+        assert all(torch.equal(g, grads[0]) for g in grads), name
+    _, f, tensors = list(every_call(amd))[2]
+    leaf = tensors[0].clone().requires_grad_()
+    losses = f(leaf, *tensors[1:])
+    (g,) = torch.autograd.grad(torch.complex(torch.zeros_like(losses), losses).conj().imag.sum(), [leaf], retain_graph=True)
+    assert torch.equal(g, torch.autograd.grad(-losses.sum(), [leaf])[0])
