@@ -699,8 +699,11 @@ int distill_args(const char* who, DistArgs& a, const void* logits, int dtype, in
         a.k2_up = std::ceil(a.k2);
         a.from_up = (float)std::exp2((double)a.k2_up - (double)a.k2);
         a.slope = A / C;
-        if (a.k1 == 0.0f) return fail(NGPT_ERANGE, "%s: softcap C=%g", who, (double)C);
+        if (a.k1 == 0.0f || !std::isfinite(a.k1) || !std::isfinite(a.k0) || !std::isfinite(a.slope))
+            return fail(NGPT_ERANGE, "%s: softcap A=%g B=%g C=%g: 1 / C, B / C or A / C outside 32-bit floats", who, (double)A, (double)B, (double)C);
     }
+    // (0 times an infinite 1 / temperature would be NaN for the largest logit)
+    if (!std::isfinite(a.k2)) return fail(NGPT_ERANGE, "%s: temperature %g: its reciprocal is not a 32-bit float", who, (double)tau);
     a.logits = logits; a.ld = ld; a.ids = ids; a.ids64 = ids_64; a.teacher = teacher; a.teacher_lse = teacher_lse; a.weight = weight;
     a.T = T; a.V = V; a.K = K; a.tau = tau;
     return NGPT_OK;

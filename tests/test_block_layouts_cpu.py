@@ -91,3 +91,12 @@ def test_dimensions_of_size_one_do_not_make_rows_uneven(rows_in_place):
         assert readable(v) and rows_in_place(v), (v.shape, v.stride())
     for v in (t[:, :2, 0], t[:, -1:, :, 3:], t[:, :1].expand(4, 3, 6, 48), t[:, :1, :5], t.transpose(0, 1)[:, :, :1]):
         assert not rows_in_place(v), (v.shape, v.stride())
+
+
+def test_distill_constants_outside_32_bit_floats_are_refused():
+    import modded_nanogpt_amd
+    lib = modded_nanogpt_amd._lib.load()
+    call = lambda tau, cap: lib.ngpt_distill_fwd(16, 0, 100, 16, 1, 16, None, None, 2, 100, 4, tau, *cap, 0, None, None)     # (no losses: -1 once these pass)
+    assert call(1.0, (0.0, 0.0, 0.0)) == -1 and call(1e-30, (0.0, 0.0, 0.0)) == -1 and call(1.0, (23.0, 5.0, 7.5)) == -1
+    assert call(1e-40, (0.0, 0.0, 0.0)) == -4 and b"reciprocal" in lib.ngpt_last_error()
+    assert call(1.0, (23.0, 5.0, 1e-40)) == -4 and call(1.0, (23.0, 1e38, 1e-3)) == -4 and call(1.0, (50.0, 0.0, 1e-38)) == -4
