@@ -47,9 +47,10 @@ __device__ __forceinline__ float act_slope(float z) {
         const float cdf = normal_cdf(z, gauss);
         return __builtin_fmaf(z * 0.3989422804014327f, gauss, cdf);
     } else if constexpr (ACT == NGPT_ACT_GELU_TANH) {
-        const float u = z * __builtin_fmaf(z * z, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
+        const float zz = fminf(z * z, 1e12f);      // (s is 0 or 1 long before; an infinite z^2 times s (1 - s) = 0 would be NaN.  z keeps a NaN)
+        const float u = z * __builtin_fmaf(zz, 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
         const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-2.0f * kLog2e * u));
-        return s + z * s * (1.0f - s) * 2.0f * __builtin_fmaf(z * z, 3.0f * 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
+        return s + z * s * (1.0f - s) * 2.0f * __builtin_fmaf(zz, 3.0f * 0.7978845608028654f * 0.044715f, 0.7978845608028654f);
     } else if constexpr (ACT == NGPT_ACT_SILU) {
         const float s = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-kLog2e * z));
         return s + z * s * (1.0f - s);

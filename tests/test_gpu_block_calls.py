@@ -3,7 +3,7 @@ formulas.  Bounds are that file's, which count roundings."""
 import pytest
 import torch
 
-from test_gpu_block import BF, D, F32, check_distill, check_linear, close, rnd, teacher_rows
+from test_gpu_block import BF, D, F32, act64, check_distill, check_linear, close, rnd, teacher_rows
 
 pytestmark = pytest.mark.gpu
 
@@ -289,3 +289,22 @@ def test_lazily_negated_tensors(amd):
     losses = f(leaf, *tensors[1:])
     (g,) = torch.autograd.grad(torch.complex(torch.zeros_like(losses), losses).conj().imag.sum(), [leaf], retain_graph=True)
     assert torch.equal(g, torch.autograd.grad(-losses.sum(), [leaf])[0])
+
+
+@pytest.mark.parametrize("act", ["none", "relu2", "gelu", "gelu_tanh", "silu"])
+def test_activations_and_slopes_at_every_bf16_value(amd, act):
+    """the type's lowest value, what masks are made of, among them; a NaN stays one"""
+    v = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).to(D).view(BF)
+    one, w, z = torch.ones(1, 1, dtype=BF, device=D), v[:, None].contiguous(), v.double()
+    y64, s64, _ = act64(z, act)
+    for M in (1, 40):                      # both kernels of small sizes
+        y = amd.linear_act(one.expand(M, 1), w, None, None, act)[-1]
+        bound = 2.0 ** -8 * y64.abs() + 8 * 2.0 ** -24 * z.abs() + 1e-37                  # the store; a few fp32 operations; no denormals
+        ok = (y == y64.to(BF)) | ((y.double() - y64).abs() <= bound)
+        assert ok[v.isfinite()].all() and y[v.isnan()].isnan().all(), (act, M, v[v.isfinite() & ~ok][:4])
+    if act == "none":
+        return
+    db = torch.ops.nanogpt.linear_act_backward(torch.ones(1, 1 << 16, dtype=BF, device=D), one, w, v[None], act, False, False, True)[2]
+    bound = 2.0 ** -8 * s64.abs() + 16 * 2.0 ** -24 * (1 + z.abs().clamp_max(100))        # (beyond 100 a smooth slope is 0 or 1)
+    ok = (db == s64.to(BF)) | ((db.double() - s64).abs() <= bound)
+    assert ok[v.isfinite()].all() and db[v.isnan()].isnan().all(), (act, v[v.isfinite() & ~ok][:4])
