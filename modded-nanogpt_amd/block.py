@@ -160,8 +160,9 @@ linear_act_op.register_autograd(_linear_backward, setup_context=_linear_setup)
 def linear_act(x: Tensor, w: Tensor, bias: Tensor | None = None, residual: Tensor | None = None, activation: str = "none") -> Tensor:
     """residual + act(x @ w.T + bias) for bf16 x [..., K], w [N, K], bias [N], residual [..., N]; fp32 accumulation, bias, activation
     and residual applied to the fp32 sums, one rounding.  `activation`: "none", "relu2" (max(z, 0)^2), "gelu", "gelu_tanh", "silu".
-    Any sizes (2^29 rows, 2^21 values in one); rows of x, w and residual may be strided.  Differentiable in x, w, bias and residual; an activation's backward keeps
-    the bf16 pre-activation."""
+    Any sizes (2^29 rows, 2^21 values in one).  Rows of x, w and residual are read in place if they are contiguous and evenly spaced, at most
+    2^21 values apart; other layouts are copied.  Differentiable in x, w, bias and residual; an activation's backward keeps
+    the bf16 pre-activation and rounds its gradient to bf16 for the two products."""
     if not is_dynamo_compiling():       # straight to the binding, which takes ordinary tensors in usable form
         act = ACTIVATIONS.get(activation)
         if act is not None:

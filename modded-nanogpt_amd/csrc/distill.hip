@@ -21,8 +21,8 @@
 //  * a sixteenth wave prepares the listed columns (normaliser, repetitions, the student's logits there) of the NEXT row and hands
 //    every one to the thread that owns the column, by a list in LDS; the owner stores it after the piece it lies in;
 //  * the next row's loads are issued before this row is reduced and written: one barrier a row.
-// Measured: 8192 rows of 50304 bf16 with softcap and 64 listed columns, loss and gradient in one pass: 324 us (1.65 GB, 5.1 TB/s: a large copy's
-// rate; 1331 us with rows in branches and the lists on the row's own waves).  1003 rows of 50257 fp32 with the rest's mass: loss 47 to 57 us
+// Measured: 8192 rows of 50304 bf16 with softcap and 64 listed columns, loss and gradient in one pass: 317 to 322 us (1.65 GB, 5.1 to 5.2 TB/s: a
+// large copy's rate; 1331 us with rows in branches and the lists on the row's own waves).  1003 rows of 50257 fp32 with the rest's mass: loss 47 to 57 us
 // (202 MB), gradient 80 us (403 MB, 5.0 TB/s).  Seven rows, loss only: 7.9 us, one row's way through one compute unit.
 #include "common.h"
 #include "host_util.h"

@@ -3,7 +3,11 @@
 //   z = x w^T + bias     x [M, K], w [N, K] bf16, bias [N], residual [M, N] optional
 //   backward: dz = dout act'(z);  dx = dz w;  dw = dz^T x;  dbias = sum of dz over the rows;  dresidual = dout
 // Products on the matrix pipe with fp32 accumulation; bias, activation and residual are applied to the fp32 sums, one rounding
-// at the store.  Training keeps z in bf16 (the activation's slope is computed from it) and feeds dz to the matrix pipe in bf16.
+// at the store.  Two more roundings to bf16 in a training step with an activation, both of which any bf16 autograd makes: z is kept in
+// bf16 for the slope (fp32 would double what a layer keeps until its backward), and dz goes to the matrix pipe in bf16 (as a sum of two
+// it would double the time of both products).  Relative error of dx and dw against 64 bits, 16384 x 1024 -> 4096: 1.66e-3 without an
+// activation (the store's own rounding), 2.41e-3 with gelu, gelu_tanh or silu (dz 1.66e-3, z 0.5e-3), 2.87e-3 with relu2, whose slope is z
+// itself; dbias, summed before dz is rounded: 1.70, 1.70 and 2.32e-3.
 #include "gemm_tn.h"
 #include "host_util.h"
 #include "launch.h"
